@@ -278,9 +278,14 @@ def _thresholds(s, n, step):
 def _code(value, scale, power, top, u):
     """The level c of top^power with value / scale * top^power between c^power and (c + 1)^power, one up where u says so."""
     r = value * torch.where(scale > 0, float(top ** power) / scale, torch.zeros_like(scale))
-    c = r.pow(1.0 / power).floor().clamp(max=top)
-    low = c.pow(power)
-    return (c + (r - low > u * ((c + 1).pow(power) - low)).double()).clamp(max=top)
+    c = (r.sqrt().sqrt() if power == 4 else r.sqrt()).floor().clamp(max=top)
+    low = _power(c, power)
+    return (c + (r - low > u * (_power(c + 1, power) - low)).double()).clamp(max=top)
+
+
+def _power(c, power):
+    """Whole numbers' squares and fourth powers, without the last digit that a library's power may lose."""
+    return (c * c) * (c * c) if power == 4 else c * c
 
 
 def _plain_adamw(s):
@@ -297,7 +302,7 @@ def _plain_adamw(s):
         S = s["scale"].double()
         k, g = s["m"].double(), g.double()
         m = b1 * (k * k.abs() * wide(S[:, 0] / 127 ** 2)) + (1 - b1) * g
-        v = b2 * (s["v"].double().pow(4) * wide(S[:, 1] / 255 ** 4)) + (1 - b2) * (g * g)
+        v = b2 * (_power(s["v"].double(), 4) * wide(S[:, 1] / 255 ** 4)) + (1 - b2) * (g * g)
         s["scale"].copy_(torch.stack([m.abs().reshape(-1, BLOCK).amax(dim=1), v.reshape(-1, BLOCK).amax(dim=1)], dim=1))
         S = s["scale"].double()
         um, uv = _thresholds(s, n, step)
@@ -311,7 +316,7 @@ def _plain_adamw(s):
     if c["bits"] == 32:
         return _adamw_outputs(s, s["m"], s["v"])
     k = s["m"].double()
-    m, v = (k * k.abs() * wide(S[:, 0] / 127 ** 2)).float(), (s["v"].double().pow(4) * wide(S[:, 1] / 255 ** 4)).float()
+    m, v = (k * k.abs() * wide(S[:, 0] / 127 ** 2)).float(), (_power(s["v"].double(), 4) * wide(S[:, 1] / 255 ** 4)).float()
     return _adamw_outputs(s, *([v[o:o + k] for o, k in zip(s["offsets"], s["sizes"])] for v in (m, v)))
 
 
