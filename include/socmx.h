@@ -549,6 +549,92 @@ int socmx_relu_bwd_colsum_f32(const float* gy, const float* y, int64_t R, int32_
 int socmx_linear_bwd_finish_f32(const float* gw_parts, int32_t S, int64_t N, const float* tail, float* gw,
                                 const float* partial, int32_t nblk, int32_t C, float* gb, socmx_stream_t stream);
 
+/* ---- layer operators: layer norm, gated scan, AdamW ---------------------------------------------------
+ * What a recurrent layer needs to be trained beside the linear / ReLU operators above.  No reference counterpart.  Element types: */
+enum { SOCMX_F32 = 0, SOCMX_BF16 = 1, SOCMX_F16 = 2 };
+/* (an unknown or unsupported type is SOCMX_E_KIND.)  Pointers need the alignment of one element only. */
+
+/*
+ * Layer norm over the last dimension:  y = (x - mean) / sqrt(var + eps) * weight + bias, all sums in f32, one rounding to `type`.
+ *   x (rows, cols) with x_stride elements between rows; y (rows, cols) dense; weight, bias (cols,) of type `wtype` (= type, or f32), each
+ *   may be NULL (ones / zeros); mean, rstd (rows,) f32 for the backward, NULL together when none follows.  1 <= cols <= 2^24.
+ * Backward: dx (rows, cols) dense, dweight, dbias (cols,) of type wtype, each may be NULL (not all); workspace:
+ *   socmx_layer_norm_bwd_workspace_floats, needed for dweight / dbias, contents undefined before and after.  The sums over rows have a
+ *   fixed order (no atomics).
+ */
+int socmx_layer_norm_fwd(int32_t type, int32_t wtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
+                         const void* weight, const void* bias, float eps, void* y, float* mean, float* rstd,
+                         socmx_stream_t stream);
+int64_t socmx_layer_norm_bwd_workspace_floats(int32_t type, int64_t rows, int64_t cols);
+int socmx_layer_norm_bwd(int32_t type, int32_t wtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
+                         const void* dy, int64_t dy_stride, const void* weight, const float* mean, const float* rstd,
+                         void* dx, void* dweight, void* dbias, float* workspace, socmx_stream_t stream);
+
+/*
+ * The gated linear recurrence  h_t = exp(log_decay_t) h_{t-1} + x_t  along the first dimension of (T, B, D): the sums with a decay that
+ * socmx_matching_target_f32 kind 1 forms with ONE rate, with a decay of its own for every step, row and gate, and gradients for all.
+ *   x, h (T, B, D) of `type`, log_decay (T, B, G) of `gate_type` (= type, or f32), G divides D: gate j decays channels j D/G ..;
+ *   the last dimension dense, the others strided (elements; 0 is fine for what is only read).  initial, final_state, dfinal, dinitial
+ *   (B, D) f32 dense, each may be NULL.  lengths (B,) int32 device or NULL: row b has min(max(lengths[b], 0), T) steps; the steps behind
+ *   them are not read, their h, dx and dlog_decay are 0 and the final state is the one before them.  reverse: from a row's last step
+ *   to its first.  A decay of 0 (log_decay = -inf, or so low that exp is below 2^-126) forgets all before it, infinities and
+ *   NaN included.  A state that is infinite under other decays stays no finite number, but may become a NaN.
+ * states: socmx_gated_scan_sizes state_floats of f32, kept from the forward for the backward (NULL when none follows).  Workspaces: floats
+ *   as socmx_gated_scan_sizes says (NULL where 0), contents undefined before and after, one for each call in flight.
+ * socmx_gated_scan_step: one step on a state (B, D) f32 that is updated in place; h (B, D) dense.
+ */
+typedef struct socmx_scan {
+  int32_t type, gate_type;
+  int32_t T, B, D, G;
+  int32_t reverse, reserved;
+  int64_t x_stride_t, x_stride_b, gate_stride_t, gate_stride_b;
+  const int32_t* lengths;
+} socmx_scan;
+int socmx_gated_scan_sizes(const socmx_scan* scan, int64_t* state_floats, int64_t* fwd_workspace_floats,
+                           int64_t* bwd_workspace_floats);
+int socmx_gated_scan_fwd(const socmx_scan* scan, const void* x, const void* log_decay, const float* initial, void* h,
+                         int64_t h_stride_t, int64_t h_stride_b, float* final_state, float* states, float* workspace,
+                         socmx_stream_t stream);
+int socmx_gated_scan_bwd(const socmx_scan* scan, const void* x, const void* log_decay, const float* states, const void* dh,
+                         int64_t dh_stride_t, int64_t dh_stride_b, const float* dfinal, void* dx, int64_t dx_stride_t,
+                         int64_t dx_stride_b, void* dlog_decay, int64_t dgate_stride_t, int64_t dgate_stride_b,
+                         float* dinitial, float* workspace, socmx_stream_t stream);
+int socmx_gated_scan_step(int32_t type, int32_t gate_type, int32_t B, int32_t D, int32_t G, const void* x, int64_t x_stride,
+                          const void* log_decay, int64_t gate_stride, float* state, int64_t state_stride, void* h,
+                          socmx_stream_t stream);
+
+/*
+ * AdamW (decoupled weight decay) over any number of tensors of one type:
+ *     m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ * tensors: HOST array, read during the call.  Weights and gradients of `type`, n elements each, dense; master: f32 weights that the update
+ *   works on, the weight getting their rounding (NULL: none; not for f32).  bits = 32: exp_avg, exp_avg_sq f32.  bits = 8: exp_avg int8 and
+ *   exp_avg_sq uint8 codes with scale (ceil(n / 256), 2) f32, m = scale0 c |c| / 127^2, v = scale1 (c / 255)^4 (csrc/socmx_adamw.hip);
+ *   codes and scales 0 are states of 0.  socmx_adamw_state_values writes what codes stand for, in f32.
+ * steps (ntensors,) f32 device: the updates each tensor has had, advanced by the call (so that a captured call counts its replays).
+ * workspace: 4 ntensors floats.  No two tensors may overlap; n may be 0 (the step is counted).
+ */
+typedef struct socmx_adamw_tensor {
+  void* p;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scale;
+  float* master;
+  int64_t n;
+} socmx_adamw_tensor;
+typedef struct socmx_adamw_state {
+  const void* exp_avg;
+  const void* exp_avg_sq;
+  const float* scale;
+  float* out_exp_avg;
+  float* out_exp_avg_sq;
+  int64_t n;
+} socmx_adamw_state;
+int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps,
+                     float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
+                     socmx_stream_t stream);
+int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t nstates, socmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

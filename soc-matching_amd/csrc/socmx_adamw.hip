@@ -1,0 +1,371 @@
+// socmx_adamw.hip -- AdamW over many tensors at once, states in 32 or in 8 bits, gfx950.
+//
+//   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by memory: with f32 weights 28 bytes an element in 32 bits, 16 in 8 bits.  A workgroup takes 4096 elements of one tensor; the
+// tensors' addresses travel in the kernel's arguments (48 tensors a launch), so a call needs no table in device memory and can be
+// captured.  Step counts stay on the device: a first launch advances them and forms the bias corrections, in 64 bits.
+//
+// STATES IN 8 BITS, per block of 256 elements of a tensor, with two f32 scales:  m = S_m c |c| / 127^2 (c in -127..127, S_m = max |m|),
+// v = S_v (c / 255)^4 (c in 0..255, S_v = max v).  The levels crowd towards zero as the values do: 1.6 % of the block's maximum
+// apart at the top for m and for sqrt(v), 2^-14 and 2^-16 of it the smallest.  An average with weight 1 - b2 = 0.001 moves by less
+// than half a level a step, so rounding to the nearest one would freeze it: a state goes to the level above with the probability
+// of its place between the two -- unbiased, so that the average keeps its mean -- where the "probability" is a 32-bit mix of the
+// element's index and the step: the same on every run, and no random numbers to carry.  Which level it is hangs on the last digits,
+// so the states are formed in 64 bits (full rate on this chip), every operation rounded by itself in the order written here: with
+// decays like 9/10 a maximum lies exactly between two f32 as often as one time in ten, and a fused product would decide otherwise
+// than the same formula elsewhere.  A positive v never becomes 0: eps alone would divide m.
+// The weight's update uses m and v as they are before they are rounded.  A block with a value that is not finite gets a NaN scale.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/socmx.h"
+#include "socmx_launch.h"
+#include "socmx_vec.h"
+
+namespace socmx {
+
+constexpr int kAdamwTensors = 48, kAdamwChunk = 4096, kAdamwBlock = 256;
+
+struct AdamwTensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float* scale;
+  float* master;
+  int64_t n;
+};
+
+struct AdamwArgs {
+  AdamwTensor tensor[kAdamwTensors];
+  int32_t first[kAdamwTensors + 1];  // the first workgroup of every tensor
+  int32_t count;
+  const float* correction;           // (count, 4): lr / (1 - b1^t), 1 / sqrt(1 - b2^t), t (as an integer), unused
+  double b1, b2;
+  float decay, eps;
+};
+
+struct AdamwValuesArgs {
+  const void* m[kAdamwTensors];
+  const void* v[kAdamwTensors];
+  const float* scale[kAdamwTensors];
+  float* out_m[kAdamwTensors];
+  float* out_v[kAdamwTensors];
+  int64_t n[kAdamwTensors];
+  int32_t first[kAdamwTensors + 1];
+  int32_t count;
+};
+
+// the tensor whose workgroups hold `block` (of several that begin there the last one: the others are empty)
+__device__ __forceinline__ int adamw_tensor(const int32_t* first, int count, int block) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= block) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// 1 - b^t in 64 bits, without cancellation
+__global__ __launch_bounds__(64) void adamw_begin_kernel(float* steps, int n, double log_b1, double log_b2, double lr, float* correction) {
+  const int i = blockIdx.x * 64 + threadIdx.x;
+  if (i >= n) return;
+  const float t = steps[i] + 1.f;
+  steps[i] = t;
+  correction[4 * i] = (float)(lr / -expm1((double)t * log_b1));
+  correction[4 * i + 1] = (float)(1.0 / sqrt(-expm1((double)t * log_b2)));
+  correction[4 * i + 2] = __uint_as_float((uint32_t)t);
+}
+
+__device__ __forceinline__ float adamw_weight(float p, float m, float v, float size, float root, float decay, float eps) {
+  float w = p * decay - size * m / (sqrtf(v) * root + eps);
+  asm("" : "+v"(w));      // a float32 from here on: a 16-bit weight is its rounding, not a second result of one mixed instruction
+  return w;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
+  const int k = adamw_tensor(a.first, a.count, blockIdx.x);
+  const AdamwTensor t = a.tensor[k];
+  const float size = a.correction[4 * k], root = a.correction[4 * k + 1];
+  const float b1 = (float)a.b1, c1 = (float)(1.0 - a.b1), b2 = (float)a.b2, c2 = (float)(1.0 - a.b2);
+  const int64_t begin = (int64_t)(blockIdx.x - a.first[k]) * kAdamwChunk;
+#pragma unroll
+  for (int r = 0; r < kAdamwChunk / 1024; ++r) {
+    const int64_t i = begin + r * 1024 + threadIdx.x * 4;
+    if (i >= t.n) return;
+    const int have = (int)std::min<int64_t>(4, t.n - i);
+    const reg_vec<T, 4> g = load_vec<T, 4>(static_cast<const T*>(t.g) + i, have);
+    const reg_vec<float, 4> m0 = load_vec<float, 4>(static_cast<float*>(t.m) + i, have), v0 = load_vec<float, 4>(static_cast<float*>(t.v) + i, have);
+    float p[4], m[4], v[4];
+    if (t.master) {
+      const reg_vec<float, 4> w = load_vec<float, 4>(t.master + i, have);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = w[e];
+    } else {
+      const reg_vec<T, 4> w = load_vec<T, 4>(static_cast<T*>(t.p) + i, have);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = w[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = b1 * m0[e] + c1 * g[e];
+      v[e] = b2 * v0[e] + c2 * (g[e] * g[e]);
+      p[e] = adamw_weight(p[e], m[e], v[e], size, root, a.decay, a.eps);
+    }
+    store_vec<float, 4>(static_cast<float*>(t.m) + i, m, have);
+    store_vec<float, 4>(static_cast<float*>(t.v) + i, v, have);
+    store_vec<T, 4>(static_cast<T*>(t.p) + i, p, have);
+    if (t.master) store_vec<float, 4>(t.master + i, p, have);
+  }
+}
+
+// two thresholds in (0, 1) from an element's place in its tensor and the step
+__device__ __forceinline__ uint32_t adamw_mix(uint32_t i, uint32_t step) {
+  uint32_t z = i * 0x9E3779B1u + step * 0xBB67AE85u;      // (odd 32-bit fractions of the golden ratio, sqrt(3) and sqrt(2))
+  z ^= z >> 16;
+  z *= 0x6A09E667u;
+  z ^= z >> 15;
+  z *= 0x9E3779B1u;
+  z ^= z >> 16;
+  return z;
+}
+__device__ __forceinline__ double adamw_threshold(uint32_t half) { return ((double)half + 0.5) * (1.0 / 65536.0); }
+
+// what the scales of 8-bit states are multiplied with when their codes are read, and divided into when codes are formed
+constexpr double kTopM = 127.0 * 127.0, kTopV = 255.0 * 255.0 * 255.0 * 255.0;
+
+// the largest of 64 lanes' bit patterns: for magnitudes this is the largest value, and NaN above infinity above all others
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = std::max(x, (uint32_t)__shfl_xor((int)x, off, 64));
+  return x;
+}
+
+// a block's scale: its maximum, or NaN where that is not finite
+__device__ __forceinline__ float adamw_scale(uint32_t bits) { return bits >= 0x7F800000u ? __builtin_nanf("") : __uint_as_float(bits); }
+
+// |m| (r = |m| / S 127^2) as a code of 0..127
+__device__ __forceinline__ int adamw_code_m(double r, double u) {
+#pragma clang fp contract(off)
+  int c = std::min((int)sqrtf((float)r), 127);
+  const double low = (double)(c * c);
+  if (r < low) --c;                                         // (the f32 root may be one off)
+  else if (r >= (double)((c + 1) * (c + 1))) ++c;
+  c = std::min(c, 127);
+  const int at = c * c;
+  return std::min(c + (r - (double)at > u * (double)(2 * c + 1) ? 1 : 0), 127);
+}
+
+// v (r = v / S 255^4) as a code of 0..255
+__device__ __forceinline__ int adamw_code_v(double r, double u) {
+#pragma clang fp contract(off)
+  auto fourth = [](int c) { return (uint32_t)(c * c) * (uint32_t)(c * c); };      // 256^4 does not fit 32 bits: c <= 255
+  int c = std::min((int)sqrtf(sqrtf((float)r)), 254);
+  if (r < (double)fourth(c)) --c;
+  else if (r >= (double)fourth(c + 1)) ++c;
+  if (c >= 255) return 255;
+  const double low = (double)fourth(c), gap = (double)(fourth(c + 1) - fourth(c));
+  return c + (r - low > u * gap ? 1 : 0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw8_kernel(const AdamwArgs a) {
+#pragma clang fp contract(off)
+  const int k = adamw_tensor(a.first, a.count, blockIdx.x);
+  const AdamwTensor t = a.tensor[k];
+  const float size = a.correction[4 * k], root = a.correction[4 * k + 1];
+  const uint32_t step = __float_as_uint(a.correction[4 * k + 2]);
+  const double b1 = a.b1, c1 = 1.0 - a.b1, b2 = a.b2, c2 = 1.0 - a.b2;
+  const int lane = threadIdx.x & 63;
+  // a wave takes a block of 256 elements at a time, four neighbouring ones a lane
+  int64_t block = (int64_t)(blockIdx.x - a.first[k]) * (kAdamwChunk / kAdamwBlock) + (threadIdx.x >> 6);
+#pragma unroll 1
+  for (int r = 0; r < kAdamwChunk / 1024; ++r, block += 4) {
+    if (block * kAdamwBlock >= t.n) return;               // (the whole wave)
+    const int64_t i = block * kAdamwBlock + lane * 4;
+    const int have = (int)std::max<int64_t>(0, std::min<int64_t>(4, t.n - i));
+    const int64_t at = have ? i : 0;
+    const reg_vec<T, 4> g = load_vec<T, 4>(static_cast<const T*>(t.g) + at, have);
+    typedef signed char i8x4 __attribute__((ext_vector_type(4), aligned(1)));
+    typedef unsigned char u8x4 __attribute__((ext_vector_type(4), aligned(1)));
+    signed char* pm = static_cast<signed char*>(t.m) + at;
+    unsigned char* pv = static_cast<unsigned char*>(t.v) + at;
+    i8x4 cm = {0, 0, 0, 0};
+    u8x4 cv = {0, 0, 0, 0};
+    if (have == 4) {
+      cm = *reinterpret_cast<i8x4*>(pm);
+      cv = *reinterpret_cast<u8x4*>(pv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < have) { cm[e] = pm[e]; cv[e] = pv[e]; }
+    }
+    float p[4];
+    if (t.master) {
+      const reg_vec<float, 4> w = load_vec<float, 4>(t.master + at, have);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = w[e];
+    } else {
+      const reg_vec<T, 4> w = load_vec<T, 4>(static_cast<T*>(t.p) + at, have);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = w[e];
+    }
+    float* scale = t.scale + 2 * block;
+    const double km = (double)scale[0] * (1.0 / kTopM), kv = (double)scale[1] * (1.0 / kTopV);
+    double m[4], v[4];
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = cm[e], s = c < 0 ? -c : c;
+      const uint32_t w = (uint32_t)cv[e] * cv[e];
+      const double ge = (double)g[e];
+      m[e] = b1 * ((double)(c * s) * km) + c1 * ge;
+      v[e] = b2 * ((double)(w * w) * kv) + c2 * (ge * ge);
+      top_m = std::max(top_m, __float_as_uint((float)m[e]) & 0x7FFFFFFFu);
+      top_v = std::max(top_v, __float_as_uint((float)v[e]));
+      p[e] = adamw_weight(p[e], (float)m[e], (float)v[e], size, root, a.decay, a.eps);
+    }
+    const float sm = adamw_scale(wave_max_bits(top_m)), sv = adamw_scale(wave_max_bits(top_v));
+    const double rm = sm > 0.f ? kTopM * (1.0 / (double)sm) : 0.0, rv = sv > 0.f ? kTopV * (1.0 / (double)sv) : 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t z = adamw_mix((uint32_t)(i + e), step);
+      const int c = adamw_code_m(fabs(m[e]) * rm, adamw_threshold(z & 0xFFFFu));
+      cm[e] = (signed char)(m[e] < 0.0 ? -c : c);
+      const int d = adamw_code_v(v[e] * rv, adamw_threshold(z >> 16));
+      cv[e] = (unsigned char)(d == 0 && v[e] > 0.0 ? 1 : d);
+    }
+    if (have == 4) {
+      *reinterpret_cast<i8x4*>(pm) = cm;
+      *reinterpret_cast<u8x4*>(pv) = cv;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < have) { pm[e] = cm[e]; pv[e] = cv[e]; }
+    }
+    if (have) {
+      store_vec<T, 4>(static_cast<T*>(t.p) + at, p, have);
+      if (t.master) store_vec<float, 4>(t.master + at, p, have);
+    }
+    if (lane == 0) {
+      scale[0] = sm;
+      scale[1] = sv;
+    }
+  }
+}
+
+// 8-bit states as the values they stand for
+__global__ __launch_bounds__(256) void adamw8_values_kernel(const AdamwValuesArgs a) {
+  const int k = adamw_tensor(a.first, a.count, blockIdx.x);
+  const int64_t n = a.n[k], begin = (int64_t)(blockIdx.x - a.first[k]) * kAdamwChunk;
+  const signed char* cm = static_cast<const signed char*>(a.m[k]);
+  const unsigned char* cv = static_cast<const unsigned char*>(a.v[k]);
+#pragma unroll
+  for (int r = 0; r < kAdamwChunk / 1024; ++r) {
+    const int64_t i = begin + r * 1024 + threadIdx.x * 4;
+    if (i >= n) return;
+    const int have = (int)std::min<int64_t>(4, n - i);
+    const float* scale = a.scale[k] + 2 * (i / kAdamwBlock);
+    const double km = (double)scale[0] * (1.0 / kTopM), kv = (double)scale[1] * (1.0 / kTopV);
+    float m[4], v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = e < have ? cm[i + e] : 0, s = c < 0 ? -c : c;
+      const uint32_t d = e < have ? cv[i + e] : 0, w = d * d;
+      m[e] = (float)((double)(c * s) * km);
+      v[e] = (float)((double)(w * w) * kv);
+    }
+    store_vec<float, 4>(a.out_m[k] + i, m, have);
+    store_vec<float, 4>(a.out_v[k] + i, v, have);
+  }
+}
+
+static inline int64_t adamw_chunks(int64_t n) { return (n + kAdamwChunk - 1) / kAdamwChunk; }
+
+}  // namespace socmx
+
+using namespace socmx;
+
+extern "C" int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps,
+                                float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                socmx_stream_t stream) {
+  if (!tensors || !steps || !workspace) return SOCMX_E_NULL;
+  if (type < SOCMX_F32 || type > SOCMX_F16 || (bits != 32 && bits != 8)) return SOCMX_E_KIND;
+  if (ntensors < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) return SOCMX_E_DIM;
+  for (int i = 0; i < ntensors; ++i) {
+    const socmx_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || t.n > (1ll << 40)) return SOCMX_E_DIM;
+    if (t.n == 0) continue;
+    if (!t.p || !t.grad || !t.exp_avg || !t.exp_avg_sq || (bits == 8 && !t.scale)) return SOCMX_E_NULL;
+    if (t.master && type == SOCMX_F32) return SOCMX_E_KIND;
+  }
+  // (b = 0: log = -inf, expm1 = -1, the correction is 1)
+  if (const int err = launch(adamw_begin_kernel, dim3((ntensors + 63) / 64), dim3(64), 0, stream, steps, (int)ntensors, log(beta1),
+                             log(beta2), lr, workspace))
+    return err;
+  int at = 0;
+  while (at < ntensors) {
+    AdamwArgs a;
+    a.b1 = beta1; a.b2 = beta2; a.decay = (float)(1.0 - lr * weight_decay); a.eps = (float)eps;
+    a.correction = workspace + 4 * (int64_t)at;
+    int64_t blocks = 0;
+    int count = 0;
+    for (; count < kAdamwTensors && at + count < ntensors; ++count) {
+      const socmx_adamw_tensor& t = tensors[at + count];
+      const int64_t more = adamw_chunks(t.n);
+      if (more > 0x3FFFFFFF) return SOCMX_E_DIM;
+      if (blocks + more > 0x7FFFFFFF) break;
+      a.tensor[count] = AdamwTensor{t.p, t.grad, t.exp_avg, t.exp_avg_sq, t.scale, t.master, t.n};
+      a.first[count] = (int32_t)blocks;
+      blocks += more;
+    }
+    a.first[count] = (int32_t)blocks;
+    a.count = count;
+    const dim3 grid((unsigned)blocks), block(256);
+    int err = 0;
+    if (blocks == 0) {
+      // (nothing but empty tensors)
+    } else if (type == SOCMX_F32)
+      err = bits == 8 ? launch(adamw8_kernel<float>, grid, block, 0, stream, a) : launch(adamw_kernel<float>, grid, block, 0, stream, a);
+    else if (type == SOCMX_BF16)
+      err = bits == 8 ? launch(adamw8_kernel<bf16_t>, grid, block, 0, stream, a) : launch(adamw_kernel<bf16_t>, grid, block, 0, stream, a);
+    else
+      err = bits == 8 ? launch(adamw8_kernel<f16_t>, grid, block, 0, stream, a) : launch(adamw_kernel<f16_t>, grid, block, 0, stream, a);
+    if (err) return err;
+    at += count;
+  }
+  return 0;
+}
+
+extern "C" int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t nstates, socmx_stream_t stream) {
+  if (!states) return SOCMX_E_NULL;
+  if (nstates < 1) return SOCMX_E_DIM;
+  for (int i = 0; i < nstates; ++i) {
+    const socmx_adamw_state& t = states[i];
+    if (t.n < 1 || t.n > (1ll << 40)) return SOCMX_E_DIM;
+    if (!t.exp_avg || !t.exp_avg_sq || !t.scale || !t.out_exp_avg || !t.out_exp_avg_sq) return SOCMX_E_NULL;
+  }
+  int at = 0;
+  while (at < nstates) {
+    AdamwValuesArgs a;
+    int64_t blocks = 0;
+    int count = 0;
+    for (; count < kAdamwTensors && at + count < nstates; ++count) {
+      const socmx_adamw_state& t = states[at + count];
+      const int64_t more = adamw_chunks(t.n);
+      if (blocks + more > 0x7FFFFFFF) break;
+      a.m[count] = t.exp_avg; a.v[count] = t.exp_avg_sq; a.scale[count] = t.scale;
+      a.out_m[count] = t.out_exp_avg; a.out_v[count] = t.out_exp_avg_sq; a.n[count] = t.n;
+      a.first[count] = (int32_t)blocks;
+      blocks += more;
+    }
+    a.first[count] = (int32_t)blocks;
+    a.count = count;
+    if (const int err = launch(adamw8_values_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a)) return err;
+    at += count;
+  }
+  return 0;
+}

@@ -96,7 +96,8 @@ def run(cfg):
         solver.gamma = cfg.method.gamma
     solver.shard = shard
     optimizer = make_optimizer(solver, nabla_V_lr=cfg.optim.nabla_V_lr, M_lr=cfg.optim.M_lr, adam_eps=cfg.optim.adam_eps,
-                               algorithm=algorithm, y0_lr=cfg.optim.y0_lr)
+                               algorithm=algorithm, y0_lr=cfg.optim.y0_lr, weight_decay=cfg.optim.get("weight_decay", 0.0),
+                               state_bits=cfg.optim.get("state_bits", None))
     optimizer.zero_grad()
     backend = cfg.get("backend", {}) or {}
     trainer = Trainer(solver, optimizer, B, normalization_const=normalization_const, algorithm=algorithm,

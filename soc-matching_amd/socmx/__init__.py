@@ -8,6 +8,8 @@ Layout:
   rollout     stochastic_trajectories (fused HIP kernel / eager torch)
   loss        SOCM loss (HIP kernels + autograd glue)
   solver      SOC_Solver
+  layers      layer norm, gated scan (with gradients; one-step form)
+  optim       AdamW over many tensors, states in 32 or 8 bits
   dist        batch sharding over GPUs (RCCL all-reduce of stats + flat gradient)
 """
 from . import _lib  # noqa: F401

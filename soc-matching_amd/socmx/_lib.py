@@ -45,6 +45,15 @@ class Control(C.Structure):
 
 CTRL_LINEAR, CTRL_CONSTANT, CTRL_TABLE = 1, 2, 3
 
+# element types of the layer operators (include/socmx.h: SOCMX_F32, SOCMX_BF16, SOCMX_F16)
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class Scan(C.Structure):
+    _fields_ = [("type", C.c_int32), ("gate_type", C.c_int32), ("T", C.c_int32), ("B", C.c_int32), ("D", C.c_int32),
+                ("G", C.c_int32), ("reverse", C.c_int32), ("reserved", C.c_int32), ("x_stride_t", C.c_int64),
+                ("x_stride_b", C.c_int64), ("gate_stride_t", C.c_int64), ("gate_stride_b", C.c_int64), ("lengths", _fp)]
+
 
 class Unet(C.Structure):
     _fields_ = [("d", C.c_int32), ("hdims", C.c_int32 * 3), ("weight", _fp * 9), ("bias", _fp * 9)]
@@ -130,6 +139,21 @@ PROTOTYPES = {
     "socmx_socm_target_bwd_net_f32": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _fp, _fp, _fp, _fp, _fp, _fp, _fp,
                                                 _fp, _fp, _fp, _fp, _fp, _fp]),
 }
+
+PROTOTYPES.update({
+    "socmx_layer_norm_fwd": (C.c_int, [C.c_int32, C.c_int32, _fp, C.c_int64, C.c_int64, C.c_int64, _fp, _fp, C.c_float, _fp, _fp,
+                                       _fp, _fp]),
+    "socmx_layer_norm_bwd_workspace_floats": (C.c_int64, [C.c_int32, C.c_int64, C.c_int64]),
+    "socmx_layer_norm_bwd": (C.c_int, [C.c_int32, C.c_int32, _fp, C.c_int64, C.c_int64, C.c_int64, _fp, C.c_int64] + [_fp] * 8),
+    "socmx_gated_scan_sizes": (C.c_int, [C.POINTER(Scan)] + [C.POINTER(C.c_int64)] * 3),
+    "socmx_gated_scan_fwd": (C.c_int, [C.POINTER(Scan), _fp, _fp, _fp, _fp, C.c_int64, C.c_int64, _fp, _fp, _fp, _fp]),
+    "socmx_gated_scan_bwd": (C.c_int, [C.POINTER(Scan), _fp, _fp, _fp, _fp, C.c_int64, C.c_int64, _fp, _fp, C.c_int64, C.c_int64, _fp,
+                                       C.c_int64, C.c_int64, _fp, _fp, _fp]),
+    "socmx_gated_scan_step": (C.c_int, [C.c_int32] * 5 + [_fp, C.c_int64, _fp, C.c_int64, _fp, C.c_int64, _fp, _fp]),
+    # (the tensors travel as host arrays of 64-bit words: 7 per socmx_adamw_tensor, 6 per socmx_adamw_state)
+    "socmx_adamw_step": (C.c_int, [C.c_int32, C.c_int32, _fp, C.c_int32, _fp, _fp] + [C.c_double] * 5 + [_fp]),
+    "socmx_adamw_state_values": (C.c_int, [_fp, C.c_int32, _fp]),
+})
 
 _lib = None
 
@@ -278,7 +302,7 @@ def variant(hdims, build=None):
     return _variants[hp]
 
 
-_STATUS_TEXT = {-1: "null pointer", -2: "bad dimension", -3: "unknown problem kind", -4: "workspace too small",
+_STATUS_TEXT = {-1: "null pointer", -2: "bad dimension", -3: "unknown problem kind or element type", -4: "workspace too small",
                 -5: "does not fit in 160 KiB of LDS (d too large for this setting / these hidden widths)"}
 
 

@@ -1,0 +1,194 @@
+"""AdamW over many tensors on the GPU, with states in 32 or in 8 bits (csrc/socmx_adamw.hip).
+
+Beside the fused Adam of the training iteration (`socmx_adam_step_f32`: one flat float32 gradient, the reference's rule without
+weight decay): decoupled weight decay, tensors wherever they lie, weights in 16 bits with float32 masters, and states of one byte each.
+`make_optimizer(weight_decay=..., state_bits=...)` (socmx/train.py) and main.py's optim.weight_decay / optim.state_bits use it.
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import SocmxError
+
+BLOCK = 256          # elements that share the two scales of 8-bit states
+
+
+def scale_rows(n):
+    """Rows of the (rows, 2) scales of a tensor of `n` elements with 8-bit states."""
+    return -(-n // BLOCK)
+
+
+def _words(rows):
+    flat = [w for row in rows for w in row]
+    return (C.c_int64 * len(flat))(*flat)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, scales=None,
+               masters=None):
+    """One AdamW update of every tensor, in place:
+
+        m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+
+    params, grads: lists of contiguous tensors of ONE type (float32, bfloat16 or float16) on one GPU.  exp_avgs, exp_avg_sqs: float32
+    tensors of the same sizes; with `scales`, 8-bit states: int8 and uint8 codes and a float32 (ceil(n / 256), 2) for each tensor of n
+    elements (zeros are states of zero; `adamw_state_values` decodes).  masters: float32 weights the update works on, the 16-bit
+    weights getting their rounding.  steps: (len(params),) float32 on the GPU, the updates so far, advanced here -- a captured call
+    counts its replays.  No two tensors may share memory; a tensor may be empty."""
+    what = "adamw_step"
+    count = len(params)
+    lists = dict(grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    if scales is not None:
+        lists["scales"] = scales
+    if masters is not None:
+        lists["masters"] = masters
+    for name, v in lists.items():
+        if len(v) != count:
+            raise SocmxError(f"{what}: {count} params and {len(v)} {name}")
+    if count == 0:
+        return
+    dev, dtype = params[0].device, params[0].dtype
+    if dev.type != "cuda":
+        raise SocmxError(f"{what}: tensors on the GPU are needed, got {dev} (there is no CPU path)")
+    if dtype not in _lib.ELEMENT_TYPES:
+        raise SocmxError(f"{what}: float32, bfloat16 or float16 weights are needed, got {dtype}")
+    if masters is not None and dtype == torch.float32:
+        raise SocmxError(f"{what}: float32 weights have no masters")
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise SocmxError(f"{what}: betas {tuple(betas)} outside [0, 1)")
+    if torch.is_tensor(lr):
+        raise SocmxError(f"{what}: lr is a number, got a tensor")
+    if tuple(steps.shape) != (count,) or steps.dtype != torch.float32 or steps.device != dev or not steps.is_contiguous():
+        raise SocmxError(f"{what}: steps is a dense ({count},) float32 on {dev}, got {tuple(steps.shape)} {steps.dtype} on {steps.device}")
+    kinds = (torch.float32, torch.float32) if scales is None else (torch.int8, torch.uint8)
+    f32 = torch.float32
+    rows = []
+    none = (None,) * count
+    for i, (p, g, m, v, s, w) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, scales or none, masters or none)):
+        n = p.numel()
+        if p.dtype != dtype or g.dtype != dtype or m.dtype != kinds[0] or v.dtype != kinds[1] or (w is not None and w.dtype != f32):
+            raise SocmxError(f"{what}: tensor {i} has types {p.dtype}, {g.dtype}, {m.dtype}, {v.dtype}"
+                             f"{'' if w is None else ', ' + str(w.dtype)}; wanted {dtype}, {dtype}, {kinds[0]}, {kinds[1]}")
+        if g.numel() != n or m.numel() != n or v.numel() != n or (w is not None and w.numel() != n):
+            raise SocmxError(f"{what}: the sizes of tensor {i} differ: {n} weights, {g.numel()} gradients, {m.numel()} and {v.numel()} states")
+        if s is not None and (tuple(s.shape) != (-(-n // BLOCK), 2) or s.dtype != f32):
+            raise SocmxError(f"{what}: the scales of tensor {i} are ({scale_rows(n)}, 2) float32, got {tuple(s.shape)} {s.dtype}")
+        for t in (p, g, m, v, s, w):
+            if t is not None and (t.device != dev or not t.is_contiguous()):
+                raise SocmxError(f"{what}: tensor {i} has a part on {t.device} with strides {t.stride()}; dense ones on {dev} are needed")
+        rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0 if s is None else s.data_ptr(),
+                     0 if w is None else w.data_ptr(), n))
+    if len({r[0] for r in rows if r[6]}) != sum(r[6] > 0 for r in rows):
+        raise SocmxError(f"{what}: the same tensor twice in params")
+    ws = torch.empty(4 * count, dtype=f32, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().socmx_adamw_step(_lib.ELEMENT_TYPES[dtype], 32 if scales is None else 8, _words(rows), count,
+                                               steps.data_ptr(), ws.data_ptr(), float(lr), float(betas[0]), float(betas[1]),
+                                               float(eps), float(weight_decay), _lib.stream_ptr(dev)), "socmx_adamw_step")
+
+
+def adamw_state_values(exp_avgs, exp_avg_sqs, scales):
+    """The values 8-bit states stand for: two lists of float32 tensors, the first and the second moments."""
+    what = "adamw_state_values"
+    if not len(exp_avgs) == len(exp_avg_sqs) == len(scales):
+        raise SocmxError(f"{what}: {len(exp_avgs)}, {len(exp_avg_sqs)} and {len(scales)} tensors")
+    ms, vs, rows = [], [], []
+    for i, (m, v, s) in enumerate(zip(exp_avgs, exp_avg_sqs, scales)):
+        if not m.is_cuda:
+            raise SocmxError(f"{what}: tensors on the GPU are needed, got {m.device} (there is no CPU path)")
+        if m.dtype != torch.int8 or v.dtype != torch.uint8 or v.shape != m.shape:
+            raise SocmxError(f"{what}: state {i} is int8 and uint8 codes of one shape, got {m.dtype} {tuple(m.shape)}, {v.dtype} {tuple(v.shape)}")
+        if tuple(s.shape) != (scale_rows(m.numel()), 2) or s.dtype != torch.float32:
+            raise SocmxError(f"{what}: the scales of state {i} are ({scale_rows(m.numel())}, 2) float32, got {tuple(s.shape)} {s.dtype}")
+        if any(t.device != exp_avgs[0].device or not t.is_contiguous() for t in (m, v, s)):
+            raise SocmxError(f"{what}: state {i} is not dense, or not on {exp_avgs[0].device}")
+        ms.append(torch.empty(m.shape, dtype=torch.float32, device=m.device))
+        vs.append(torch.empty(m.shape, dtype=torch.float32, device=m.device))
+        if m.numel():
+            rows.append((m.data_ptr(), v.data_ptr(), s.data_ptr(), ms[-1].data_ptr(), vs[-1].data_ptr(), m.numel()))
+    if rows:
+        dev = exp_avgs[0].device
+        with _lib.on_device(dev):
+            _lib.check(_lib.lib().socmx_adamw_state_values(_words(rows), len(rows), _lib.stream_ptr(dev)), "socmx_adamw_state_values")
+    return ms, vs
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step is one call of `adamw_step` for each type of weights in a group (48 tensors a launch).
+
+    state_bits: 32 (float32 states) or 8 (one byte a state, two float32 for 256 elements).  master_weights: keep float32 weights for 16-bit
+    parameters (a 16-bit weight does not see updates below 2^-9 of it).  The state is that of torch.optim.AdamW -- "step", "exp_avg",
+    "exp_avg_sq" -- and, where there are any, "scale" and "master".  Parameters without a gradient are left alone.  Step counts live
+    on the GPU, so step() can be captured in a graph once the state exists (one eager step); a learning rate is part of the capture."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, master_weights=True):
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise SocmxError(f"AdamW: lr {lr}, eps {eps} and weight_decay {weight_decay} are not negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise SocmxError(f"AdamW: betas {tuple(betas)} outside [0, 1)")
+        if state_bits not in (8, 32):
+            raise SocmxError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights))
+
+    def _new_state(self, p, group):
+        if not p.is_cuda:
+            raise SocmxError(f"AdamW: parameters on the GPU are needed, got {p.device} (there is no CPU path)")
+        if torch.cuda.is_current_stream_capturing():
+            raise SocmxError("AdamW: the state of a parameter would be created inside a capture: take one step before it")
+        st = self.state[p]
+        st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+        kinds = (torch.float32, torch.float32) if group["state_bits"] == 32 else (torch.int8, torch.uint8)
+        for name, kind in zip(("exp_avg", "exp_avg_sq"), kinds):
+            st[name] = torch.zeros(p.shape, dtype=kind, device=p.device)
+        if group["state_bits"] == 8:
+            st["scale"] = torch.zeros(scale_rows(p.numel()), 2, dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype != torch.float32:
+            st["master"] = p.detach().to(torch.float32).contiguous()
+        return st
+
+    def load_state_dict(self, state_dict):
+        """torch casts what it loads to the parameters' type: codes, masters and float32 states of 16-bit weights are taken as they are."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            for name, v in state_dict["state"].get(i, {}).items():
+                kind = torch.float32 if name == "step" or torch.is_tensor(v) and v.is_floating_point() else None
+                self.state[p][name] = torch.as_tensor(v).detach().clone().to(device=p.device, dtype=kind)
+
+    def _steps(self, found, dev):
+        """The step counts of these parameters as one tensor: their "step" entries are its elements."""
+        base = found[0][1]["step"]._base
+        if base is not None and base.dim() == 1 and base.numel() == len(found) and base.dtype == torch.float32:
+            at = base.data_ptr()
+            if all(st["step"].data_ptr() == at + 4 * i for i, (_, st) in enumerate(found)):
+                return base
+        if torch.cuda.is_current_stream_capturing():
+            raise SocmxError("AdamW: a capture needs a step with the same parameters before it")
+        base = torch.stack([st["step"].reshape(()).to(device=dev, dtype=torch.float32) for _, st in found])
+        for i, (_, st) in enumerate(found):
+            st["step"] = base[i]
+        return base
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            kinds = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise SocmxError("AdamW: a sparse gradient")
+                st = self.state.get(p) or self._new_state(p, group)
+                kinds.setdefault((p.dtype, p.device, "scale" in st, "master" in st), []).append((p, st))
+            for (_, dev, small, master), found in kinds.items():
+                adamw_step([p for p, _ in found], [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in found],
+                           [st["exp_avg"] for _, st in found], [st["exp_avg_sq"] for _, st in found], self._steps(found, dev),
+                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           scales=[st["scale"] for _, st in found] if small else None,
+                           masters=[st["master"] for _, st in found] if master else None)
+        return loss

@@ -24,8 +24,13 @@ def compute_EMA(value, EMA_value, EMA_coeff=0.01, itr=0):
     return EMA_coeff * value + (1 - EMA_coeff) * EMA_value
 
 
-def make_optimizer(solver, nabla_V_lr=1e-4, M_lr=1e-2, adam_eps=1e-4, algorithm="SOCM", y0_lr=1e-2):
-    """Adam with the per-algorithm parameter groups of main.py:174-238."""
+def make_optimizer(solver, nabla_V_lr=1e-4, M_lr=1e-2, adam_eps=1e-4, algorithm="SOCM", y0_lr=1e-2,
+                   weight_decay=0.0, state_bits=None):
+    """Adam with the per-algorithm parameter groups of main.py:174-238.
+
+    Not in the reference: weight_decay > 0 or state_bits (32 or 8) give AdamW (socmx/optim.py) over the same groups; parameters of a
+    single element (gamma, gamma2, gamma3, y0) are exponents and offsets, not weights, and are never decayed.  On the CPU (32 bits
+    only) that is torch.optim.AdamW."""
     sde = solver.neural_sde
     if algorithm == "SOCM":
         groups = [{"params": sde.nabla_V.parameters()},
@@ -41,6 +46,20 @@ def make_optimizer(solver, nabla_V_lr=1e-4, M_lr=1e-2, adam_eps=1e-4, algorithm=
         groups = [{"params": solver.parameters()}]
     # one fused multi-tensor kernel per group on the GPU (same update rule; ~20 launches fewer per iteration)
     on_gpu = next(sde.parameters()).is_cuda
+    if weight_decay or state_bits is not None:
+        split = []
+        for g in groups:
+            params = [g["params"]] if torch.is_tensor(g["params"]) else list(g["params"])
+            for single in (False, True):
+                part = [p for p in params if (p.numel() == 1) is single]
+                if part:
+                    split.append(dict(g, params=part, weight_decay=0.0 if single else weight_decay))
+        if on_gpu:
+            from .optim import AdamW
+            return AdamW(split, lr=nabla_V_lr, eps=adam_eps, weight_decay=weight_decay, state_bits=state_bits or 32)
+        if state_bits == 8:
+            raise ValueError("make_optimizer: states in 8 bits need a GPU")
+        return torch.optim.AdamW(split, lr=nabla_V_lr, eps=adam_eps, weight_decay=weight_decay)
     return torch.optim.Adam(groups, lr=nabla_V_lr, eps=adam_eps, fused=True if on_gpu else None)
 
 
