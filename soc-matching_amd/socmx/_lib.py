@@ -189,6 +189,23 @@ def lib():
     return _lib
 
 
+_binding = None
+
+
+def torch_binding():
+    """The layer operators on torch tensors (csrc/socmx_torch.cpp, built beside the library).  Raises SocmxError when it is missing."""
+    global _binding
+    if _binding is None:
+        base = lib()
+        try:
+            from . import _torch
+        except ImportError as e:
+            raise SocmxError(f"{os.path.join(_HERE, '_torch.so')} cannot be loaded ({e}): build it with `make -C soc-matching_amd/csrc`") from e
+        _torch.bind_library(base._name, SocmxError)
+        _binding = _torch
+    return _binding
+
+
 # ---- architecture variants ---------------------------------------------------------------------------------------------
 # libsocmx.so carries constexpr-specialised rollout / control-network-backward kernels for the reference's default
 # arch.hdims = [256,128,64] (configs/soc.yaml:33-35) and a descriptor-driven form for everything else (~1.6x slower per

@@ -4,8 +4,6 @@ Beside the fused Adam of the training iteration (`socmx_adam_step_f32`: one flat
 weight decay): decoupled weight decay, tensors wherever they lie, weights in 16 bits with float32 masters, and states of one byte each.
 `make_optimizer(weight_decay=..., state_bits=...)` (socmx/train.py) and main.py's optim.weight_decay / optim.state_bits use it.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -19,11 +17,6 @@ def scale_rows(n):
     return -(-n // BLOCK)
 
 
-def _words(rows):
-    flat = [w for row in rows for w in row]
-    return (C.c_int64 * len(flat))(*flat)
-
-
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, scales=None,
                masters=None):
     """One AdamW update of every tensor, in place:
@@ -35,82 +28,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     elements (zeros are states of zero; `adamw_state_values` decodes).  masters: float32 weights the update works on, the 16-bit
     weights getting their rounding.  steps: (len(params),) float32 on the GPU, the updates so far, advanced here -- a captured call
     counts its replays.  No two tensors may share memory; a tensor may be empty."""
-    what = "adamw_step"
-    count = len(params)
-    lists = dict(grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
-    if scales is not None:
-        lists["scales"] = scales
-    if masters is not None:
-        lists["masters"] = masters
-    for name, v in lists.items():
-        if len(v) != count:
-            raise SocmxError(f"{what}: {count} params and {len(v)} {name}")
-    if count == 0:
-        return
-    dev, dtype = params[0].device, params[0].dtype
-    if dev.type != "cuda":
-        raise SocmxError(f"{what}: tensors on the GPU are needed, got {dev} (there is no CPU path)")
-    if dtype not in _lib.ELEMENT_TYPES:
-        raise SocmxError(f"{what}: float32, bfloat16 or float16 weights are needed, got {dtype}")
-    if masters is not None and dtype == torch.float32:
-        raise SocmxError(f"{what}: float32 weights have no masters")
-    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-        raise SocmxError(f"{what}: betas {tuple(betas)} outside [0, 1)")
     if torch.is_tensor(lr):
-        raise SocmxError(f"{what}: lr is a number, got a tensor")
-    if tuple(steps.shape) != (count,) or steps.dtype != torch.float32 or steps.device != dev or not steps.is_contiguous():
-        raise SocmxError(f"{what}: steps is a dense ({count},) float32 on {dev}, got {tuple(steps.shape)} {steps.dtype} on {steps.device}")
-    kinds = (torch.float32, torch.float32) if scales is None else (torch.int8, torch.uint8)
-    f32 = torch.float32
-    rows = []
-    none = (None,) * count
-    for i, (p, g, m, v, s, w) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, scales or none, masters or none)):
-        n = p.numel()
-        if p.dtype != dtype or g.dtype != dtype or m.dtype != kinds[0] or v.dtype != kinds[1] or (w is not None and w.dtype != f32):
-            raise SocmxError(f"{what}: tensor {i} has types {p.dtype}, {g.dtype}, {m.dtype}, {v.dtype}"
-                             f"{'' if w is None else ', ' + str(w.dtype)}; wanted {dtype}, {dtype}, {kinds[0]}, {kinds[1]}")
-        if g.numel() != n or m.numel() != n or v.numel() != n or (w is not None and w.numel() != n):
-            raise SocmxError(f"{what}: the sizes of tensor {i} differ: {n} weights, {g.numel()} gradients, {m.numel()} and {v.numel()} states")
-        if s is not None and (tuple(s.shape) != (-(-n // BLOCK), 2) or s.dtype != f32):
-            raise SocmxError(f"{what}: the scales of tensor {i} are ({scale_rows(n)}, 2) float32, got {tuple(s.shape)} {s.dtype}")
-        for t in (p, g, m, v, s, w):
-            if t is not None and (t.device != dev or not t.is_contiguous()):
-                raise SocmxError(f"{what}: tensor {i} has a part on {t.device} with strides {t.stride()}; dense ones on {dev} are needed")
-        rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0 if s is None else s.data_ptr(),
-                     0 if w is None else w.data_ptr(), n))
-    if len({r[0] for r in rows if r[6]}) != sum(r[6] > 0 for r in rows):
-        raise SocmxError(f"{what}: the same tensor twice in params")
-    ws = torch.empty(4 * count, dtype=f32, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().socmx_adamw_step(_lib.ELEMENT_TYPES[dtype], 32 if scales is None else 8, _words(rows), count,
-                                               steps.data_ptr(), ws.data_ptr(), float(lr), float(betas[0]), float(betas[1]),
-                                               float(eps), float(weight_decay), _lib.stream_ptr(dev)), "socmx_adamw_step")
+        raise SocmxError("adamw_step: lr is a number, got a tensor")
+    _lib.torch_binding().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, scales, masters)
 
 
 def adamw_state_values(exp_avgs, exp_avg_sqs, scales):
     """The values 8-bit states stand for: two lists of float32 tensors, the first and the second moments."""
-    what = "adamw_state_values"
-    if not len(exp_avgs) == len(exp_avg_sqs) == len(scales):
-        raise SocmxError(f"{what}: {len(exp_avgs)}, {len(exp_avg_sqs)} and {len(scales)} tensors")
-    ms, vs, rows = [], [], []
-    for i, (m, v, s) in enumerate(zip(exp_avgs, exp_avg_sqs, scales)):
-        if not m.is_cuda:
-            raise SocmxError(f"{what}: tensors on the GPU are needed, got {m.device} (there is no CPU path)")
-        if m.dtype != torch.int8 or v.dtype != torch.uint8 or v.shape != m.shape:
-            raise SocmxError(f"{what}: state {i} is int8 and uint8 codes of one shape, got {m.dtype} {tuple(m.shape)}, {v.dtype} {tuple(v.shape)}")
-        if tuple(s.shape) != (scale_rows(m.numel()), 2) or s.dtype != torch.float32:
-            raise SocmxError(f"{what}: the scales of state {i} are ({scale_rows(m.numel())}, 2) float32, got {tuple(s.shape)} {s.dtype}")
-        if any(t.device != exp_avgs[0].device or not t.is_contiguous() for t in (m, v, s)):
-            raise SocmxError(f"{what}: state {i} is not dense, or not on {exp_avgs[0].device}")
-        ms.append(torch.empty(m.shape, dtype=torch.float32, device=m.device))
-        vs.append(torch.empty(m.shape, dtype=torch.float32, device=m.device))
-        if m.numel():
-            rows.append((m.data_ptr(), v.data_ptr(), s.data_ptr(), ms[-1].data_ptr(), vs[-1].data_ptr(), m.numel()))
-    if rows:
-        dev = exp_avgs[0].device
-        with _lib.on_device(dev):
-            _lib.check(_lib.lib().socmx_adamw_state_values(_words(rows), len(rows), _lib.stream_ptr(dev)), "socmx_adamw_state_values")
-    return ms, vs
+    return _lib.torch_binding().adamw_state_values(exp_avgs, exp_avg_sqs, scales)
 
 
 class AdamW(torch.optim.Optimizer):

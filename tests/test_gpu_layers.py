@@ -437,6 +437,18 @@ def test_gated_scan_refusals():
             bad()
 
 
+def test_a_second_derivative_is_refused():
+    """Not silently left out: differentiating a gradient raises."""
+    x = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    a = -torch.rand(5, 2, 4, device=DEV)
+    for y in (layers.layer_norm(x), layers.gated_scan(x, a)[0]):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(g.sum(), x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad((g * x).sum(), x)
+
+
 # ---- AdamW -------------------------------------------------------------------------------------------------------------------
 def mix(i, step):
     """The two thresholds of element i at this step (csrc/socmx_adamw.hip)."""
