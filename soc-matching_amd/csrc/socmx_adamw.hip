@@ -79,8 +79,9 @@ __global__ __launch_bounds__(64) void adamw_begin_kernel(float* steps, int n, do
   correction[4 * i + 2] = __uint_as_float((uint32_t)t);
 }
 
+// (the hardware's root and reciprocal, each within one step of f32: two of the update's two dozen roundings)
 __device__ __forceinline__ float adamw_weight(float p, float m, float v, float size, float root, float decay, float eps) {
-  float w = p * decay - size * m / (sqrtf(v) * root + eps);
+  float w = p * decay - size * m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * root + eps);
   asm("" : "+v"(w));      // a float32 from here on: a 16-bit weight is its rounding, not a second result of one mixed instruction
   return w;
 }
@@ -132,128 +133,161 @@ __device__ __forceinline__ uint32_t adamw_mix(uint32_t i, uint32_t step) {
   z ^= z >> 16;
   return z;
 }
-__device__ __forceinline__ double adamw_threshold(uint32_t half) { return ((double)half + 0.5) * (1.0 / 65536.0); }
 
 // what the scales of 8-bit states are multiplied with when their codes are read, and divided into when codes are formed
 constexpr double kTopM = 127.0 * 127.0, kTopV = 255.0 * 255.0 * 255.0 * 255.0;
 
 // the largest of 64 lanes' bit patterns: for magnitudes this is the largest value, and NaN above infinity above all others
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x = std::max(x, (uint32_t)__shfl_xor((int)x, off, 64));
-  return x;
+  auto dpp = [](uint32_t v, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true); };
+  x = std::max(x, dpp(x, std::integral_constant<int, 0xB1>{}));     // quad_perm [1,0,3,2]
+  x = std::max(x, dpp(x, std::integral_constant<int, 0x4E>{}));     // quad_perm [2,3,0,1]
+  x = std::max(x, dpp(x, std::integral_constant<int, 0x141>{}));    // mirror of 8 lanes
+  x = std::max(x, dpp(x, std::integral_constant<int, 0x140>{}));    // mirror of 16 lanes
+  x = std::max(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+  return std::max(x, (uint32_t)__shfl_xor((int)x, 32, 64));
 }
 
 // a block's scale: its maximum, or NaN where that is not finite
 __device__ __forceinline__ float adamw_scale(uint32_t bits) { return bits >= 0x7F800000u ? __builtin_nanf("") : __uint_as_float(bits); }
 
-// |m| (r = |m| / S 127^2) as a code of 0..127
-__device__ __forceinline__ int adamw_code_m(double r, double u) {
-#pragma clang fp contract(off)
-  int c = std::min((int)sqrtf((float)r), 127);
-  const double low = (double)(c * c);
-  if (r < low) --c;                                         // (the f32 root may be one off)
-  else if (r >= (double)((c + 1) * (c + 1))) ++c;
-  c = std::min(c, 127);
-  const int at = c * c;
-  return std::min(c + (r - (double)at > u * (double)(2 * c + 1) ? 1 : 0), 127);
+// A code is c or c + 1 with c^n <= y < (c + 1)^n, the upper one where y - c^n > u ((c + 1)^n - c^n), u = (2 k + 1) / 2^17.  The f32 root,
+// taken a little low, gives c or the level below it: the test is made there and once more a level up, and the code is that level and
+// one for each test that holds -- the same code either way, with no case to tell apart.  `half`: k.
+constexpr float kRootLow = 1.f - 4.8e-7f;                           // (four steps of f32; root and conversion are within two)
+
+// (a product of values that fit 24 bits is one full-rate instruction, which looks at no other bits)
+__device__ __forceinline__ uint32_t mul_small(uint32_t a, uint32_t b) {
+  return (a & 0xFFFFFFu) * (b & 0xFFFFFFu);
 }
 
-// v (r = v / S 255^4) as a code of 0..255
-__device__ __forceinline__ int adamw_code_v(double r, double u) {
+// y = |m| / S 127^2.  In whole numbers: 2^17 y, rounded up, is above a whole threshold exactly where y is.
+__device__ __forceinline__ int adamw_code_m(double y_scaled, uint32_t half) {
+  const uint32_t y = (uint32_t)__builtin_ceil(y_scaled);            // at most 2^17 127^2 and a bit: below 2^31
+  const uint32_t c = (uint32_t)(__builtin_amdgcn_sqrtf((float)y) * (0.00276213586400995125f * kRootLow));      // 2^-8.5
+  const uint32_t rest = y - (mul_small(c, c) << 17), gap = 2 * c + 1, odd = 2 * half + 1, first = mul_small(odd, gap);
+  const uint32_t second = (gap << 17) + first + 2 * odd;            // the gap, and u of the next one, which is 2 wider
+  return std::min((int)(c + (rest > first) + (rest > second)), 127);
+}
+
+// y = v / S 255^4: differences of fourth powers need 64 bits, which hold every term exactly
+__device__ __forceinline__ int adamw_code_v(double y, uint32_t half) {
 #pragma clang fp contract(off)
-  auto fourth = [](int c) { return (uint32_t)(c * c) * (uint32_t)(c * c); };      // 256^4 does not fit 32 bits: c <= 255
-  int c = std::min((int)sqrtf(sqrtf((float)r)), 254);
-  if (r < (double)fourth(c)) --c;
-  else if (r >= (double)fourth(c + 1)) ++c;
-  if (c >= 255) return 255;
-  const double low = (double)fourth(c), gap = (double)(fourth(c + 1) - fourth(c));
-  return c + (r - low > u * gap ? 1 : 0);
+  const uint32_t c = (uint32_t)(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) * kRootLow);           // at most 254
+  const uint32_t c2 = mul_small(c, c), d2 = c2 + 2 * c + 1, e2 = d2 + 2 * c + 3;
+  const uint32_t c4 = mul_small(c2, c2), d4 = mul_small(d2, d2), e4 = mul_small(e2, e2);    // (256^4 wraps to 0, its difference does not)
+  const double u = (double)(2 * half + 1) * (1.0 / 131072.0), rest = y - (double)c4, gap = (double)(d4 - c4);
+  return std::min((int)(c + (rest > u * gap) + (rest > gap + u * (double)(e4 - d4))), 255);
+}
+
+template <typename T>
+struct Adamw8Block {                 // what a lane needs of its four elements
+  reg_vec<T, 4> g, p16;
+  reg_vec<float, 4> p32;
+  uint32_t cm, cv;
+  float sm, sv;
+};
+typedef uint32_t packed_codes __attribute__((aligned(1)));
+
+// `have` of the four elements from `i` on (4 and nothing else where FULL)
+template <typename T, bool FULL>
+__device__ __forceinline__ Adamw8Block<T> adamw8_load(const AdamwTensor& t, int64_t block, int64_t i, int have) {
+  Adamw8Block<T> b;
+  if (FULL) have = 4;
+  const int64_t at = FULL || have ? i : 0;
+  b.g = load_vec<T, 4>(static_cast<const T*>(t.g) + at, have);
+  if (t.master) b.p32 = load_vec<float, 4>(t.master + at, have);
+  else b.p16 = load_vec<T, 4>(static_cast<T*>(t.p) + at, have);
+  const unsigned char *pm = static_cast<unsigned char*>(t.m) + at, *pv = static_cast<unsigned char*>(t.v) + at;
+  if (have == 4) {
+    b.cm = *reinterpret_cast<const packed_codes*>(pm);
+    b.cv = *reinterpret_cast<const packed_codes*>(pv);
+  } else {
+    b.cm = b.cv = 0;
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < have) { b.cm |= (uint32_t)pm[e] << (8 * e); b.cv |= (uint32_t)pv[e] << (8 * e); }
+  }
+  b.sm = t.scale[2 * block];
+  b.sv = t.scale[2 * block + 1];
+  return b;
+}
+
+struct Adamw8Step { double b1, c1, b2, c2; float size, root, decay, eps; uint32_t step; };
+
+template <typename T, bool FULL>
+__device__ __forceinline__ void adamw8_block(const AdamwTensor& t, const Adamw8Step& h, const Adamw8Block<T>& now, int64_t block, int64_t i, int have) {
+#pragma clang fp contract(off)
+  if (FULL) have = 4;
+  const double km = (double)now.sm * (1.0 / kTopM), kv = (double)now.sv * (1.0 / kTopV);
+  float p[4];
+  double m[4], v[4];
+  uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = (int)(now.cm << (24 - 8 * e)) >> 24;
+    const uint32_t d = (now.cv >> (8 * e)) & 255u, w = mul_small(d, d);
+    const double ge = (double)now.g[e];
+    m[e] = h.b1 * ((double)__mul24(c, c < 0 ? -c : c) * km) + h.c1 * ge;
+    v[e] = h.b2 * ((double)mul_small(w, w) * kv) + h.c2 * (ge * ge);
+    top_m = std::max(top_m, __float_as_uint((float)m[e]) & 0x7FFFFFFFu);
+    top_v = std::max(top_v, __float_as_uint((float)v[e]));
+    p[e] = adamw_weight(t.master ? now.p32[e] : now.p16[e], (float)m[e], (float)v[e], h.size, h.root, h.decay, h.eps);
+  }
+  const float sm = adamw_scale(wave_max_bits(top_m)), sv = adamw_scale(wave_max_bits(top_v));
+  const double rm = sm > 0.f ? kTopM * (1.0 / (double)sm) * 131072.0 : 0.0, rv = sv > 0.f ? kTopV * (1.0 / (double)sv) : 0.0;
+  uint32_t cm = 0, cv = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t z = adamw_mix((uint32_t)(i + e), h.step);
+    const int c = adamw_code_m(fabs(m[e]) * rm, z & 0xFFFFu), d = adamw_code_v(v[e] * rv, z >> 16);
+    cm |= ((uint32_t)(m[e] < 0.0 ? -c : c) & 255u) << (8 * e);
+    cv |= (uint32_t)(d == 0 && v[e] > 0.0 ? 1 : d) << (8 * e);
+  }
+  if (have) {
+    unsigned char *pm = static_cast<unsigned char*>(t.m) + i, *pv = static_cast<unsigned char*>(t.v) + i;
+    if (have == 4) {
+      *reinterpret_cast<packed_codes*>(pm) = cm;
+      *reinterpret_cast<packed_codes*>(pv) = cv;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < have) { pm[e] = (unsigned char)(cm >> (8 * e)); pv[e] = (unsigned char)(cv >> (8 * e)); }
+    }
+    store_vec<T, 4>(static_cast<T*>(t.p) + i, p, have);
+    if (t.master) store_vec<float, 4>(t.master + i, p, have);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    t.scale[2 * block] = sm;
+    t.scale[2 * block + 1] = sv;
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8_kernel(const AdamwArgs a) {
-#pragma clang fp contract(off)
   const int k = adamw_tensor(a.first, a.count, blockIdx.x);
   const AdamwTensor t = a.tensor[k];
-  const float size = a.correction[4 * k], root = a.correction[4 * k + 1];
-  const uint32_t step = __float_as_uint(a.correction[4 * k + 2]);
-  const double b1 = a.b1, c1 = 1.0 - a.b1, b2 = a.b2, c2 = 1.0 - a.b2;
-  const int lane = threadIdx.x & 63;
-  // a wave takes a block of 256 elements at a time, four neighbouring ones a lane
-  int64_t block = (int64_t)(blockIdx.x - a.first[k]) * (kAdamwChunk / kAdamwBlock) + (threadIdx.x >> 6);
+  const Adamw8Step h = {a.b1, 1.0 - a.b1, a.b2, 1.0 - a.b2, a.correction[4 * k], a.correction[4 * k + 1], a.decay, a.eps,
+                        __float_as_uint(a.correction[4 * k + 2])};
+  // a wave takes a block of 256 elements at a time, four neighbouring ones a lane; the next block's loads are in flight meanwhile
+  const int64_t full = t.n / kAdamwBlock, first = (int64_t)(blockIdx.x - a.first[k]) * (kAdamwChunk / kAdamwBlock);
+  const int64_t end = std::min<int64_t>(full, first + kAdamwChunk / kAdamwBlock);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t block = first + wave;
+  if (block < end) {
+    Adamw8Block<T> next = adamw8_load<T, true>(t, block, block * kAdamwBlock + lane * 4, 4);
 #pragma unroll 1
-  for (int r = 0; r < kAdamwChunk / 1024; ++r, block += 4) {
-    if (block * kAdamwBlock >= t.n) return;               // (the whole wave)
+    for (; block < end; block += 4) {
+      const Adamw8Block<T> now = next;
+      if (block + 4 < end) next = adamw8_load<T, true>(t, block + 4, (block + 4) * kAdamwBlock + lane * 4, 4);
+      adamw8_block<T, true>(t, h, now, block, block * kAdamwBlock + lane * 4, 4);
+    }
+  }
+  // the tensor's last block, where it is not a whole one
+  if (block == full && block < first + kAdamwChunk / kAdamwBlock && full * kAdamwBlock < t.n) {
     const int64_t i = block * kAdamwBlock + lane * 4;
     const int have = (int)std::max<int64_t>(0, std::min<int64_t>(4, t.n - i));
-    const int64_t at = have ? i : 0;
-    const reg_vec<T, 4> g = load_vec<T, 4>(static_cast<const T*>(t.g) + at, have);
-    typedef signed char i8x4 __attribute__((ext_vector_type(4), aligned(1)));
-    typedef unsigned char u8x4 __attribute__((ext_vector_type(4), aligned(1)));
-    signed char* pm = static_cast<signed char*>(t.m) + at;
-    unsigned char* pv = static_cast<unsigned char*>(t.v) + at;
-    i8x4 cm = {0, 0, 0, 0};
-    u8x4 cv = {0, 0, 0, 0};
-    if (have == 4) {
-      cm = *reinterpret_cast<i8x4*>(pm);
-      cv = *reinterpret_cast<u8x4*>(pv);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < have) { cm[e] = pm[e]; cv[e] = pv[e]; }
-    }
-    float p[4];
-    if (t.master) {
-      const reg_vec<float, 4> w = load_vec<float, 4>(t.master + at, have);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = w[e];
-    } else {
-      const reg_vec<T, 4> w = load_vec<T, 4>(static_cast<T*>(t.p) + at, have);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = w[e];
-    }
-    float* scale = t.scale + 2 * block;
-    const double km = (double)scale[0] * (1.0 / kTopM), kv = (double)scale[1] * (1.0 / kTopV);
-    double m[4], v[4];
-    uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = cm[e], s = c < 0 ? -c : c;
-      const uint32_t w = (uint32_t)cv[e] * cv[e];
-      const double ge = (double)g[e];
-      m[e] = b1 * ((double)(c * s) * km) + c1 * ge;
-      v[e] = b2 * ((double)(w * w) * kv) + c2 * (ge * ge);
-      top_m = std::max(top_m, __float_as_uint((float)m[e]) & 0x7FFFFFFFu);
-      top_v = std::max(top_v, __float_as_uint((float)v[e]));
-      p[e] = adamw_weight(p[e], (float)m[e], (float)v[e], size, root, a.decay, a.eps);
-    }
-    const float sm = adamw_scale(wave_max_bits(top_m)), sv = adamw_scale(wave_max_bits(top_v));
-    const double rm = sm > 0.f ? kTopM * (1.0 / (double)sm) : 0.0, rv = sv > 0.f ? kTopV * (1.0 / (double)sv) : 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t z = adamw_mix((uint32_t)(i + e), step);
-      const int c = adamw_code_m(fabs(m[e]) * rm, adamw_threshold(z & 0xFFFFu));
-      cm[e] = (signed char)(m[e] < 0.0 ? -c : c);
-      const int d = adamw_code_v(v[e] * rv, adamw_threshold(z >> 16));
-      cv[e] = (unsigned char)(d == 0 && v[e] > 0.0 ? 1 : d);
-    }
-    if (have == 4) {
-      *reinterpret_cast<i8x4*>(pm) = cm;
-      *reinterpret_cast<u8x4*>(pv) = cv;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < have) { pm[e] = cm[e]; pv[e] = cv[e]; }
-    }
-    if (have) {
-      store_vec<T, 4>(static_cast<T*>(t.p) + at, p, have);
-      if (t.master) store_vec<float, 4>(t.master + at, p, have);
-    }
-    if (lane == 0) {
-      scale[0] = sm;
-      scale[1] = sv;
-    }
+    adamw8_block<T, false>(t, h, adamw8_load<T, false>(t, block, i, have), block, i, have);
   }
 }
 

@@ -418,6 +418,14 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
                              ws.data_ptr<float>(), lr, b1, b2, eps, weight_decay, l.stream), "socmx_adamw_step");
 }
 
+// a dense tensor of its own over a part of a buffer's storage (which lives as long as one of them does)
+Tensor part_of(const Tensor& flat, int64_t offset, at::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 std::pair<Tensors, Tensors> adamw_state_values(const Tensors& ms, const Tensors& vs, const Tensors& scales) {
   const char* what = "adamw_state_values";
   const size_t count = ms.size();
@@ -426,6 +434,11 @@ std::pair<Tensors, Tensors> adamw_state_values(const Tensors& ms, const Tensors&
   if (count == 0) return out;
   const at::Device dev = ms[0].device();
   on_gpu(what, ms[0]);
+  out.first.reserve(count);
+  out.second.reserve(count);
+  int64_t total = 0, at = 0;           // (one allocation for all first, one for all second moments, each at a multiple of 64 bytes)
+  for (const Tensor& m : ms) total += (m.numel() + 15) / 16 * 16;
+  const Tensor flat_m = empty({total}, at::kFloat, dev), flat_v = empty({total}, at::kFloat, dev);
   std::vector<socmx_adamw_state> rows;
   for (size_t i = 0; i < count; ++i) {
     const Tensor &m = ms[i], &v = vs[i], &s = scales[i];
@@ -436,8 +449,9 @@ std::pair<Tensors, Tensors> adamw_state_values(const Tensors& ms, const Tensors&
       refuse(what, ": the scales of state ", i, " are (", blocks, ", 2) float32, got ", shape(s), " ", s.scalar_type());
     for (const Tensor* t : {&m, &v, &s})
       if (t->device() != dev || !t->is_contiguous()) refuse(what, ": state ", i, " is not dense, or not on ", dev);
-    out.first.push_back(empty(m.sizes(), at::kFloat, dev));
-    out.second.push_back(empty(m.sizes(), at::kFloat, dev));
+    out.first.push_back(part_of(flat_m, at, m.sizes()));
+    out.second.push_back(part_of(flat_v, at, m.sizes()));
+    at += (n + 15) / 16 * 16;
     if (n)
       rows.push_back(socmx_adamw_state{pointer(m), pointer(v), s.data_ptr<float>(), out.first.back().data_ptr<float>(),
                                        out.second.back().data_ptr<float>(), n});
