@@ -291,29 +291,51 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamwArgs a) {
   }
 }
 
-// 8-bit states as the values they stand for
+// 8-bit states as the values they stand for: 2 bytes in, 8 out an element
 __global__ __launch_bounds__(256) void adamw8_values_kernel(const AdamwValuesArgs a) {
   const int k = adamw_tensor(a.first, a.count, blockIdx.x);
-  const int64_t n = a.n[k], begin = (int64_t)(blockIdx.x - a.first[k]) * kAdamwChunk;
-  const signed char* cm = static_cast<const signed char*>(a.m[k]);
+  const int64_t n = a.n[k], begin = (int64_t)(blockIdx.x - a.first[k]) * kAdamwChunk + threadIdx.x * 4;
+  const unsigned char* cm = static_cast<const unsigned char*>(a.m[k]);
   const unsigned char* cv = static_cast<const unsigned char*>(a.v[k]);
-#pragma unroll
-  for (int r = 0; r < kAdamwChunk / 1024; ++r) {
-    const int64_t i = begin + r * 1024 + threadIdx.x * 4;
-    if (i >= n) return;
-    const int have = (int)std::min<int64_t>(4, n - i);
-    const float* scale = a.scale[k] + 2 * (i / kAdamwBlock);
-    const double km = (double)scale[0] * (1.0 / kTopM), kv = (double)scale[1] * (1.0 / kTopV);
+  const float* scale = a.scale[k];
+  float *out_m = a.out_m[k], *out_v = a.out_v[k];
+  constexpr int R = kAdamwChunk / 1024;
+  auto put = [&](int64_t i, uint32_t bm, uint32_t bv, float sm, float sv, int have) {
+    const double km = (double)sm * (1.0 / kTopM), kv = (double)sv * (1.0 / kTopV);
     float m[4], v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int c = e < have ? cm[i + e] : 0, s = c < 0 ? -c : c;
-      const uint32_t d = e < have ? cv[i + e] : 0, w = d * d;
-      m[e] = (float)((double)(c * s) * km);
-      v[e] = (float)((double)(w * w) * kv);
+      const int c = (int)(bm << (24 - 8 * e)) >> 24;
+      const uint32_t d = (bv >> (8 * e)) & 255u, w = mul_small(d, d);
+      m[e] = (float)((double)__mul24(c, c < 0 ? -c : c) * km);
+      v[e] = (float)((double)mul_small(w, w) * kv);
     }
-    store_vec<float, 4>(a.out_m[k] + i, m, have);
-    store_vec<float, 4>(a.out_v[k] + i, v, have);
+    store_vec<float, 4>(out_m + i, m, have);
+    store_vec<float, 4>(out_v + i, v, have);
+  };
+  if ((int64_t)(blockIdx.x - a.first[k] + 1) * kAdamwChunk <= n) {
+    uint32_t bm[R], bv[R];
+    float sm[R], sv[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t i = begin + r * 1024;
+      bm[r] = *reinterpret_cast<const packed_codes*>(cm + i);
+      bv[r] = *reinterpret_cast<const packed_codes*>(cv + i);
+      sm[r] = scale[2 * (i / kAdamwBlock)];
+      sv[r] = scale[2 * (i / kAdamwBlock) + 1];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) put(begin + r * 1024, bm[r], bv[r], sm[r], sv[r], 4);
+    return;
+  }
+  for (int64_t i = begin; i < n && i < begin + kAdamwChunk; i += 1024) {
+    const int have = (int)std::min<int64_t>(4, n - i);
+    uint32_t bm = 0, bv = 0;
+    for (int e = 0; e < have; ++e) {
+      bm |= (uint32_t)cm[i + e] << (8 * e);
+      bv |= (uint32_t)cv[i + e] << (8 * e);
+    }
+    put(i, bm, bv, scale[2 * (i / kAdamwBlock)], scale[2 * (i / kAdamwBlock) + 1], have);
   }
 }
 
