@@ -580,7 +580,8 @@ int socmx_layer_norm_bwd(int32_t type, int32_t wtype, const void* x, int64_t row
  *   to its first.  A decay of 0 (log_decay = -inf, or so low that exp is below 2^-126) forgets all before it, infinities and
  *   NaN included.  A state that is infinite under other decays stays no finite number, but may become a NaN.
  * states: socmx_gated_scan_sizes state_floats of f32, kept from the forward for the backward (NULL when none follows).  Workspaces: floats
- *   as socmx_gated_scan_sizes says (NULL where 0), contents undefined before and after, one for each call in flight.
+ *   as socmx_gated_scan_sizes says (NULL where 0; at a multiple of 8 bytes), contents undefined before and after, one for each call in
+ *   flight.
  * socmx_gated_scan_step: one step on a state (B, D) f32 that is updated in place; h (B, D) dense.
  */
 typedef struct socmx_scan {

@@ -10,23 +10,33 @@
 // precision) and r = 1, any other as q = exp(alpha) and r = 0: a h + x is q h + x, plus r h, two fused operations.  q = 0 (exp flushes
 // what is below 2^-126) is a gate that forgets: whatever stood before it, infinities and NaN included, is replaced, not multiplied.
 //
-// RUNS.  A step is an affine map, so a run of steps is one: h -> exp(S) h + l with S the sum of its alphas and l its result from zero --
-// the same form, applied with the code of a step.  A wave owns 64 V channels and a run of steps, and walks it alone, U steps at a time
-// with the next U in flight: no barrier, nothing but the state between two steps.  Where the channels do not fill the chip, time is
-// cut into runs: a first launch forms every run's (S, l), W of them a workgroup, and the composition of those W; the second composes the
-// workgroups in front of its own, then the waves, and walks its run from the state it found.  x and alpha are read twice for that,
-// the second time mostly out of the last-level cache: the second launch takes the runs in the opposite order.  (A form whose
-// waves met in LDS every 64 steps took 329 us against 215 at (4096, 8, 2048) bf16 with 32 gates and padded rows, forward and backward, and
-// 450 against 435 at (65536, 1, 640) f32.)
+// ONE READ.  A step is an affine map, so a run of steps is one: h -> exp(S) h + l with S the sum of its alphas and l its result from zero --
+// the same form, applied with the code of a step.  A workgroup owns 64 V channels and a chunk of W U steps, a wave U of them, in registers.
+// Every wave forms its run's (S, l); the waves meet in LDS; the workgroup leaves its chunk's (q, l) in memory for the chunks behind it, takes
+// those in front of it from there, and its waves walk their steps from the state they find.  So x and alpha are read once and h is
+// written once, however few channels there are.
+//   Who waits for whom: chunks are dealt out by a ticket in the order of the steps, so a chunk waits only for workgroups that have started
+// and that leave their (q, l) without waiting for anybody.  A chunk takes at most kGroup - 1 of them, in order; the state at every kGroup-th
+// chunk is left by the chunk in front of it, which is the one chain along time.  What is composed with what does not depend on who comes
+// first: the same bits on every run.  A word in memory is its own flag: it is set to kEmpty by a launch before this one, written once by one
+// 64-bit store, and read until it is something else -- no fence, which would write back the cache of a whole die.  A wait that lasts
+// kPolls reads (about a second) ends in NaN: the launch ends whatever happens.
 //
-// THE BACKWARD walks the steps from the end.  It rebuilds U steps of h at a time in f32 from the states that the forward leaves every
-// U steps (f32, 1 / U of h) -- h itself, rounded to 16 bits, would put its rounding into dalpha.  A gate shared by several channels: their
+// THE BACKWARD is the same from the end.  It rebuilds a wave's U steps of h in f32 from the state that the forward leaves in front of them
+// (f32, 1 / U of h) -- h itself, rounded to 16 bits, would put its rounding into dalpha.  A gate shared by several channels: their
 // products are summed across the lanes in a fixed order, gates wider than a wave leave one partial sum a wave for another launch.  No
-// atomics: the same bits on every run.  Bound by memory: x, alpha (, dh) in, h (dx, dalpha) out.
+// floating-point atomics.
+//
+// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 118 us (4.3 TB/s of x, alpha, h and states) + 172 us (5.0): memory, a copy of
+// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 84 us (3.5 TB/s) + 131 us (3.3); rows that are on average 3/4
+// full 72 + 111, of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 20 + 28.
+// Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57.  U = 16, W = 8 and
+// kGroup = 16 were the best or within 2 % of it among U 4, 8, 16, W 4, 8, 16 and groups of 16, 32; chunks wait for each other 3 to 7 % of the time.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "../../include/socmx.h"
 #include "socmx_launch.h"
@@ -40,13 +50,16 @@ struct ScanArgs {
   const float *initial, *dfinal;     // (B, D), nullable (zeros)
   float *final, *dinitial;           // (B, D), nullable
   float* state;                      // (ceil(T / U), B D): the state in front of every U-th step; written by the forward when not NULL
-  float* run;                        // (chunks, 1 + W, 2, B D): q and l of a workgroup's steps, then of each of its waves' (chunked only)
+  uint64_t* word;                    // (chunks, B D): q and l of every chunk; then (ceil(chunks / kGroup), B D) floats: the state at its first
+  float* mark;                       //   chunk; then the ticket (more than one chunk only)
+  uint32_t* ticket;
   float* part;                       // (T, B G, segments): partial sums of dalpha (gates wider than a wave only)
   const int32_t* lengths;            // (B,), nullable
   int64_t xt, xb, at, ab, ht, hb, dht, dhb;   // elements between steps / rows of x, alpha, h, dh
   int64_t dxt, dxb, dat, dab;                 // of dx, dalpha
   int T, B, D, G, reverse;
-  int steps, chunks;                 // steps of a run (a multiple of U), workgroups of W runs along time
+  int chunks;
+  uint32_t blocks;                   // workgroups a chunk
 };
 
 // ---- gates --------------------------------------------------------------------------------------------------------------------
@@ -78,9 +91,27 @@ __device__ __forceinline__ float gate_times(float q, float r, float h) {
   if (CUT) h = q == 0.f ? 0.f : h;
   return fmaf(r, h, q * h);
 }
-__device__ __forceinline__ float gate_apply(float q, float h, float x) { return gate_apply<true>(q, gate_keeps(q), h, x); }
 
-constexpr int kScanW = 8, kScanU = 8;
+// Runs of steps: the sum of their alphas (-inf if a gate forgets, whatever the others are), the gate of all of them -- one that forgets only if a
+// single one does: a state that is NaN in front of gates whose product is below 2^-126 stays so -- and the run applied to a state.  From a
+// state of zero it is its own result, also where the gates' product is beyond f32.
+__device__ __forceinline__ float run_join(float s, float t) {
+  constexpr float cut = -__builtin_inff();
+  return s == cut || t == cut ? cut : s + t;
+}
+__device__ __forceinline__ float run_gate(float sum) {
+  const float q = gate_of(sum);
+  return q == 0.f && sum != -__builtin_inff() ? 1.17549435e-38f : q;
+}
+__device__ __forceinline__ float run_apply(float q, float h, float l) {
+  q = h == 0.f ? 0.f : q;
+  return gate_apply<true>(q, gate_keeps(q), h, l);
+}
+
+constexpr int kScanW = 8, kScanU = 16, kScanTile = kScanW * kScanU, kGroup = 16;
+constexpr int kPolls = 1 << 20;
+constexpr uint64_t kEmpty = ~0ull;
+constexpr uint32_t kNoState = ~0u;
 
 // Which channels a lane owns.  V neighbouring ones of one row; where a gate is shared and its products have to be summed
 // (GROUPED), the lanes of a gate are neighbours and no gate straddles two waves unless it is wider than one.
@@ -93,7 +124,7 @@ struct ScanLane {
 };
 
 template <int V, bool GROUPED>
-__device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a) {
+__device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a, uint32_t block) {
   ScanLane l;
   const int lane = threadIdx.x & 63, per = a.D / a.G;
   l.group = 0; l.seg = 0; l.at = 0; l.lanes = 1; l.first = 1;
@@ -101,15 +132,15 @@ __device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a) {
     const int wide = per / V;        // lanes of a gate
     if (wide <= 64) {
       const int fit = 64 / wide;
-      l.group = (int64_t)blockIdx.x * fit + lane / wide;
+      l.group = (int64_t)block * fit + lane / wide;
       l.at = lane % wide;
       l.lanes = wide;
       l.live = lane / wide < fit && l.group < (int64_t)a.B * a.G;
       l.c = l.at * V;
     } else {
       const int segs = (wide + 63) / 64;
-      l.group = blockIdx.x / segs;
-      l.seg = blockIdx.x % segs;
+      l.group = block / segs;
+      l.seg = block % segs;
       l.at = lane;
       l.lanes = min(64, wide - l.seg * 64);
       l.live = lane < l.lanes;
@@ -122,7 +153,7 @@ __device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a) {
     l.c += l.gate * per;
     l.ch = (int64_t)l.b * a.D + l.c;
   } else {
-    l.ch = ((int64_t)blockIdx.x * 64 + lane) * V;
+    l.ch = ((int64_t)block * 64 + lane) * V;
     l.live = l.ch < (int64_t)a.B * a.D;
     if (!l.live) l.ch = 0;
     l.b = (int)(l.ch / a.D);
@@ -134,25 +165,37 @@ __device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a) {
   return l;
 }
 
-// where a wave's steps end: at `end`, or at the first multiple of U behind the last step that one of its rows has
-__device__ __forceinline__ int scan_stop(const ScanLane& l, int begin, int end) {
-  int most = l.live ? l.len : 0;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
-  return max(begin, min(end, (most + kScanU - 1) / kScanU * kScanU));
-}
-
-// zeros at the steps [from, to) of a lane's V channels (or its gates), which lie behind the lengths
-template <typename T, int V>
-__device__ __forceinline__ void scan_clear(T* origin, int64_t st, int from, int to) {
-  const float zero[V] = {};
-  for (int k = from; k < to; ++k) store_vec<T, V>(origin + (int64_t)k * st, zero);
-}
-
 // the address of a row's step 0, and the distance from a step to the next one, in the row's direction
 template <typename T>
 __device__ __forceinline__ T* scan_origin(T* p, const ScanArgs& a, const ScanLane& l, int64_t st, int64_t sb, int c) {
   return p + (int64_t)l.b * sb + c + (a.reverse && l.len > 0 ? (int64_t)(l.len - 1) * st : 0);
+}
+
+// What the compiler is not to see through.  It would keep, from one pass over the steps to the next, the sixteen addresses of every array,
+// the elements widened to f32 and what is derived from the gates: registers without which twice the waves fit.
+template <typename T>
+__device__ __forceinline__ void scan_next(T*& p, int64_t d) {
+  p += d;
+  asm("" : "+v"(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void scan_forget(reg_vec<T, V>& r) {
+  if constexpr (sizeof(T) * V == 8) {
+    uint64_t w = __builtin_bit_cast(uint64_t, r);
+    asm("" : "+v"(w));
+    r = __builtin_bit_cast(reg_vec<T, V>, w);
+  } else if constexpr (sizeof(T) * V == 4) {
+    uint32_t w = __builtin_bit_cast(uint32_t, r);
+    asm("" : "+v"(w));
+    r = __builtin_bit_cast(reg_vec<T, V>, w);
+  }
+}
+template <int NA>
+__device__ __forceinline__ void scan_forget(float (&q)[kScanU][NA]) {
+#pragma unroll
+  for (int u = 0; u < kScanU; ++u)
+#pragma unroll
+    for (int i = 0; i < NA; ++i) asm("" : "+v"(q[u][i]));
 }
 
 // U steps from step k0 on, V values each; nothing is read behind the length
@@ -161,366 +204,465 @@ __device__ __forceinline__ void scan_load(reg_vec<T, V> (&out)[kScanU], const T*
   const T* p = origin + (int64_t)k0 * d;
   if (full) {
 #pragma unroll
-    for (int u = 0; u < kScanU; ++u) out[u] = load_vec<T, V>(p + u * d);
+    for (int u = 0; u < kScanU; ++u, scan_next(p, d)) out[u] = load_vec<T, V>(p);
   } else {
 #pragma unroll
-    for (int u = 0; u < kScanU; ++u)
-      if (k0 + u < len) out[u] = load_vec<T, V>(p + u * d);
+    for (int u = 0; u < kScanU; ++u, scan_next(p, d))
+      if (k0 + u < len) out[u] = load_vec<T, V>(p);
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void scan_values(float (&out)[kScanU][V], const reg_vec<T, V> (&raw)[kScanU], int k0, int len, bool full) {
-  if (full) {
-#pragma unroll
-    for (int u = 0; u < kScanU; ++u)
-#pragma unroll
-      for (int i = 0; i < V; ++i) out[u][i] = raw[u][i];
-  } else {
-#pragma unroll
-    for (int u = 0; u < kScanU; ++u)
-#pragma unroll
-      for (int i = 0; i < V; ++i) out[u][i] = k0 + u < len ? raw[u][i] : 0.f;
-  }
+template <int... U>
+__device__ __forceinline__ void gate_hand(float (&q)[kScanU][1], float g, std::integer_sequence<int, U...>) {
+  ((q[U][0] = dpp_move<0x150 + U>(g)), ...);       // (lane U of the row to all of them)
 }
 
-// q and r of U steps; whether one of this wave's gates forgets
-template <typename TA, int NA>
-__device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&r)[kScanU][NA], const reg_vec<TA, NA> (&raw)[kScanU], int k0, int len,
-                                           bool full) {
+// q of U steps and the sum of their alphas (-inf once a gate forgets); whether one of this wave's gates does.  origin: alpha at step 0.
+// ROW: the 16 lanes of a row share their gate.  Lane u of a row takes step u -- one load and one gate instead of sixteen -- and hands it to the
+// others.
+template <typename TA, int NA, bool ROW>
+__device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&sum)[NA], const TA* origin, int64_t d, int k0, int len, bool full) {
   bool cut = false;
-#pragma unroll
-  for (int u = 0; u < kScanU; ++u)
+  if constexpr (ROW) {
+    static_assert(NA == 1 && kScanU == 16, "a gate for a row of 16 lanes, a step for each of them");
+    const int u = threadIdx.x & 15;
+    const bool in = full || k0 + u < len;
+    float g = kGateKeeps, s = 0.f;
+    if (in) {
+      s = (float)origin[(int64_t)(k0 + u) * d];
+      g = gate_of(s);
+      cut = g == 0.f;
+    }
+    const float any = lanes_sum<16>(cut ? 1.f : 0.f);
+    sum[0] = lanes_sum<16>(s);
+    if (any > 0.f) sum[0] = -__builtin_inff();
+    gate_hand(q, g, std::make_integer_sequence<int, kScanU>{});
+  } else {
+    reg_vec<TA, NA> raw[kScanU];
+    scan_load<TA, NA>(raw, origin, d, k0, len, full);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      q[u][i] = gate_of(raw[u][i]);
-      if (!full && k0 + u >= len) q[u][i] = kGateKeeps;
-      r[u][i] = gate_keeps(q[u][i]);
-      cut |= q[u][i] == 0.f;
+      bool zero = false;
+      sum[i] = 0.f;
+#pragma unroll
+      for (int u = 0; u < kScanU; ++u) {
+        const bool in = full || k0 + u < len;
+        const float alpha = raw[u][i];
+        q[u][i] = in ? gate_of(alpha) : kGateKeeps;
+        sum[i] += in ? alpha : 0.f;
+        zero |= q[u][i] == 0.f;
+      }
+      if (zero) sum[i] = -__builtin_inff();
+      cut |= zero;
     }
+  }
   return __any(cut);
 }
 
-// the sum of a run's alphas, -inf once a gate forgets
-template <typename TA, int NA>
-__device__ __forceinline__ void scan_sum(float (&sum)[NA], const float (&q)[kScanU][NA], const reg_vec<TA, NA> (&raw)[kScanU], int k0, int len,
-                                         bool full) {
+// ---- the chunks in front ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float plain_nan(float v) { return v != v ? __builtin_nanf("") : v; }      // (never a bit pattern that means empty)
+
+__device__ __forceinline__ void leave_word(uint64_t* p, float q, float l) {
+  const uint64_t v = (uint64_t)__float_as_uint(plain_nan(q)) | (uint64_t)__float_as_uint(l) << 32;
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void leave_state(float* p, float s) {
+  __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(plain_nan(s)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// N words each lane with `need` waits for
+template <int N>
+__device__ __forceinline__ void take_words(float (&q)[N], float (&l)[N], const uint64_t* p, bool need) {
+  uint64_t v[N];
+  for (int left = kPolls;; --left) {
+    bool missing = false;
 #pragma unroll
-  for (int u = 0; u < kScanU; ++u)
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const float alpha = !full && k0 + u >= len ? 0.f : (float)raw[u][i];
-      sum[i] += q[u][i] == 0.f ? -__builtin_inff() : alpha;
+    for (int i = 0; i < N; ++i) {
+      v[i] = need ? __hip_atomic_load(const_cast<uint64_t*>(p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+      missing |= need && v[i] == kEmpty;
     }
-}
-
-// the state in front of (behind, for the backward) a wave's run, from the runs of the workgroups and then the waves before it
-template <int V>
-__device__ __forceinline__ void scan_compose(float (&s)[V], const ScanArgs& a, int64_t ch, int chunk, int wave, int first_chunk, int first_wave) {
-  const int64_t C = (int64_t)a.B * a.D, row = 2 * C, step = (1 + kScanW) * row;
-  const int by = first_chunk <= chunk ? 1 : -1;
-#pragma unroll 4
-  for (int j = first_chunk; j != chunk; j += by) {
-    const float* p = a.run + j * step + ch;
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = gate_apply(p[i], s[i], p[C + i]);
+    if (!__any(missing) || left == 0) break;
+    __builtin_amdgcn_s_sleep(0);
   }
-  const int wby = first_wave <= wave ? 1 : -1;
-  for (int w = first_wave; w != wave; w += wby) {
-    const float* p = a.run + chunk * step + (1 + w) * row + ch;
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = gate_apply(p[i], s[i], p[C + i]);
+  for (int i = 0; i < N; ++i) {
+    q[i] = __uint_as_float((uint32_t)v[i]);        // (kEmpty after kPolls reads: NaN)
+    l[i] = __uint_as_float((uint32_t)(v[i] >> 32));
   }
 }
+__device__ __forceinline__ float take_state(const float* p, bool need) {
+  uint32_t v;
+  for (int left = kPolls;; --left) {
+    v = need ? __hip_atomic_load(reinterpret_cast<uint32_t*>(const_cast<float*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    if (!__any(need && v == kNoState) || left == 0) break;
+    __builtin_amdgcn_s_sleep(0);
+  }
+  return __uint_as_float(v);
+}
 
-// a wave's run (S, l) to memory, and the composition of its workgroup's: in the order of the steps, or against it (back)
+__global__ __launch_bounds__(256) void gated_scan_clear_kernel(uint64_t* word, int64_t words, uint32_t* ticket) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < words) word[i] = kEmpty;                 // (two empty states a word in the second part)
+  if (i == 0) *ticket = 0;
+}
+
 template <int V, int NA>
-__device__ __forceinline__ void scan_runs(const ScanArgs& a, const ScanLane& l, int chunk, const float (&sum)[NA], const float (&run)[V], bool back) {
-  __shared__ float exs[kScanW][NA][64], exl[kScanW][V][64];
+struct ScanMeet {                                  // where the waves of a workgroup meet
+  float q[kScanW][NA][64], sum[kScanW][NA][64], l[kScanW][V][64];       // the waves' runs
+  float pq[kGroup - 1][V][64], pl[kGroup - 1][V][64];   // the chunks in front, back to the last marked one
+  float in[V][64];                                 // the state in front of (behind) the chunk
+  uint32_t ticket;
+};
+
+// the number of this workgroup among all of its launch, in the order in which they start
+template <int V, int NA>
+__device__ __forceinline__ uint32_t scan_ticket(const ScanArgs& a, ScanMeet<V, NA>& m) {
+  if (a.chunks == 1) return blockIdx.x;
+  if (threadIdx.x == 0) m.ticket = atomicAdd(a.ticket, 1u);
+  __syncthreads();
+  return m.ticket;
+}
+
+// The waves' runs (sum, run: this wave's) into the meeting place, and the chunk's (q, l) into memory, for the chunks behind chunk `chunk`
+// (counted in the walk's direction).  The first V waves do that, for one of a lane's channels each.  BACK: the waves' order within the chunk
+// is the opposite one.
+template <int V, int NA, bool BACK>
+__device__ __forceinline__ void scan_leave(ScanMeet<V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, const float (&sum)[NA],
+                                           const float (&run)[V], float& chunk_q, float& chunk_l) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    m.q[wave][i][lane] = run_gate(sum[i]);
+    m.sum[wave][i][lane] = sum[i];
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) m.l[wave][i][lane] = run[i];
+  __syncthreads();
+  chunk_q = chunk_l = 0.f;
+  if (wave < V) {
+    const int gate = NA == 1 ? 0 : wave;
+#pragma unroll
+    for (int k = 0; k < kScanW; ++k) {
+      const int w = BACK ? kScanW - 1 - k : k;
+      chunk_q = run_join(chunk_q, m.sum[w][gate][lane]);
+      chunk_l = run_apply(m.q[w][gate][lane], chunk_l, m.l[w][wave][lane]);
+    }
+    chunk_q = run_gate(chunk_q);
+    if (chunk + 1 < a.chunks && (chunk + 1) % kGroup != 0 && l.live)
+      leave_word(a.word + chunk * ((int64_t)a.B * a.D) + l.ch + wave, chunk_q, chunk_l);
+  }
+}
+
+// the state in front of the chunk into m.in; first: the state in front of all steps
+template <int V, int NA>
+__device__ __forceinline__ void scan_take(ScanMeet<V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, float chunk_q, float chunk_l,
+                                          const float* first) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t C = (int64_t)a.B * a.D;
-  float* p = a.run + (int64_t)chunk * (1 + kScanW) * 2 * C + l.ch;
-#pragma unroll
-  for (int i = 0; i < NA; ++i) exs[wave][i][lane] = sum[i];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    exl[wave][i][lane] = run[i];
-    if (l.live) {
-      p[(1 + wave) * 2 * C + i] = gate_of(sum[NA == 1 ? 0 : i]);
-      p[(1 + wave) * 2 * C + C + i] = run[i];
-    }
-  }
-  __syncthreads();
-  if (wave == 0 && l.live) {
+  const int marked = chunk / kGroup * kGroup;
+  for (int j = wave; j < chunk - marked; j += kScanW) {
+    float q[V], t[V];
+    take_words<V>(q, t, a.word + (marked + j) * C + l.ch, l.live);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float s = 0.f, all = 0.f;
-#pragma unroll
-      for (int k = 0; k < kScanW; ++k) {
-        const int w = back ? kScanW - 1 - k : k;
-        const float one = exs[w][NA == 1 ? 0 : i][lane];
-        s = gate_apply(gate_of(one), s, exl[w][i][lane]);
-        all += one;
-      }
-      p[i] = gate_of(all);
-      p[C + i] = s;
+      m.pq[j][i][lane] = q[i];
+      m.pl[j][i][lane] = t[i];
     }
   }
-}
-
-// the first launch of a forward in chunks: the runs of all of them but the last
-template <typename T, typename TA, int V, int NA>
-__global__ __launch_bounds__(64 * kScanW) void gated_scan_fwd_runs_kernel(const ScanArgs a) {
-  const int wave = threadIdx.x >> 6, chunk = blockIdx.y;
-  const ScanLane l = scan_lane<V, false>(a);
-  const int64_t dx = a.reverse ? -a.xt : a.xt, da = a.reverse ? -a.at : a.at;
-  const T* x0 = scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c);
-  const TA* a0 = scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c);
-  const int begin = (chunk * kScanW + wave) * a.steps, end = min(begin + a.steps, a.T);
-  float sum[NA] = {}, run[V] = {};
-  reg_vec<T, V> rx[kScanU];
-  reg_vec<TA, NA> ra[kScanU];
-  auto fetch = [&](int k0) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    scan_load<T, V>(rx, x0, dx, k0, l.len, full);
-    scan_load<TA, NA>(ra, a0, da, k0, l.len, full);
-  };
-  const int stop = scan_stop(l, begin, end);
-  if (begin < stop) fetch(begin);
-  for (int k0 = begin; k0 < stop; k0 += kScanU) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    float x[kScanU][V], q[kScanU][NA], r[kScanU][NA];
-    scan_values<T, V>(x, rx, k0, l.len, full);
-    const bool cut = scan_gates<TA, NA>(q, r, ra, k0, l.len, full);
-    scan_sum<TA, NA>(sum, q, ra, k0, l.len, full);
-    if (k0 + kScanU < stop) fetch(k0 + kScanU);
-    auto walk = [&](auto CUT) {
-#pragma unroll
-      for (int u = 0; u < kScanU; ++u)
-#pragma unroll
-        for (int i = 0; i < V; ++i) run[i] = gate_apply<decltype(CUT)::value>(q[u][NA == 1 ? 0 : i], r[u][NA == 1 ? 0 : i], run[i], x[u][i]);
-    };
-    if (cut) walk(std::true_type{}); else walk(std::false_type{});
+  float s = 0.f;
+  if (wave < V) {
+    if (marked > 0) s = take_state(a.mark + marked / kGroup * C + l.ch + wave, l.live);
+    else if (first && l.live) s = first[l.ch + wave];
   }
-  scan_runs<V, NA>(a, l, chunk, sum, run, false);
+  __syncthreads();
+  if (wave < V) {
+#pragma unroll 4
+    for (int j = 0; j < chunk - marked; ++j) s = run_apply(m.pq[j][wave][lane], s, m.pl[j][wave][lane]);
+    m.in[wave][lane] = s;
+    if (chunk + 1 < a.chunks && (chunk + 1) % kGroup == 0 && l.live)
+      leave_state(a.mark + (chunk + 1) / kGroup * C + l.ch + wave, run_apply(chunk_q, s, chunk_l));
+  }
+  __syncthreads();
 }
 
-template <typename T, typename TA, int V, int NA>
-__global__ __launch_bounds__(64 * kScanW) void gated_scan_fwd_kernel(const ScanArgs a) {
-  const int wave = threadIdx.x >> 6, chunk = a.chunks - 1 - blockIdx.y;
-  const ScanLane l = scan_lane<V, false>(a);
+// a wave's own state: the chunk's, past the waves in front
+template <int V, int NA, bool BACK>
+__device__ __forceinline__ void scan_own_state(float (&h)[V], const ScanMeet<V, NA>& m) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < V; ++i) h[i] = m.in[i][lane];
+  for (int k = 0; k < (BACK ? kScanW - 1 - wave : wave); ++k) {
+    const int w = BACK ? kScanW - 1 - k : k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = run_apply(m.q[w][NA == 1 ? 0 : i][lane], h[i], m.l[w][i][lane]);
+  }
+}
+
+// (4 waves a SIMD, 97 registers at most: 6 of them at 80 gave 90 us for 84)
+template <typename T, typename TA, int V, int NA, bool ROW>
+__global__ __launch_bounds__(64 * kScanW, 4) void gated_scan_fwd_kernel(const ScanArgs a) {
+  __shared__ ScanMeet<V, NA> meet;
+  const uint32_t number = scan_ticket(a, meet);
+  const int wave = threadIdx.x >> 6, chunk = number / a.blocks;
+  const ScanLane l = scan_lane<V, false>(a, number % a.blocks);
   const int64_t C = (int64_t)a.B * a.D;
   const int64_t dx = a.reverse ? -a.xt : a.xt, da = a.reverse ? -a.at : a.at, dh = a.reverse ? -a.ht : a.ht;
-  const T* x0 = scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c);
-  const TA* a0 = scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c);
-  T* h0 = scan_origin(static_cast<T*>(a.h), a, l, a.ht, a.hb, l.c);
-  T* pad = static_cast<T*>(a.h) + (int64_t)l.b * a.hb + l.c;        // steps behind the length lie at their own index
-  const int begin = (chunk * kScanW + wave) * a.steps, end = min(begin + a.steps, a.T);
-  if (begin >= end) return;
+  const int k0 = (chunk * kScanW + wave) * kScanU;
+  const bool full = __all(k0 + kScanU <= l.len), none = !__any(l.live && k0 < l.len);
   reg_vec<T, V> rx[kScanU];
-  reg_vec<TA, NA> ra[kScanU];
-  auto fetch = [&](int k0) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    scan_load<T, V>(rx, x0, dx, k0, l.len, full);
-    scan_load<TA, NA>(ra, a0, da, k0, l.len, full);
-  };
-  const int stop = scan_stop(l, begin, end);
-  if (begin < stop) fetch(begin);
-  float h[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) h[i] = a.initial && l.live ? a.initial[l.ch + i] : 0.f;
-  if (begin > 0) scan_compose<V>(h, a, l.ch, chunk, wave, 0, 0);
-  for (int k0 = begin; k0 < stop; k0 += kScanU) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    float x[kScanU][V], q[kScanU][NA], r[kScanU][NA];
-    scan_values<T, V>(x, rx, k0, l.len, full);
-    const bool cut = scan_gates<TA, NA>(q, r, ra, k0, l.len, full);
-    if (k0 + kScanU < stop) fetch(k0 + kScanU);
-    if (a.state && l.live) store_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch, h);
-    auto walk = [&](auto CUT, auto FULL) {
-#pragma unroll
-      for (int u = 0; u < kScanU; ++u) {
-        const int k = k0 + u;
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = gate_apply<decltype(CUT)::value>(q[u][NA == 1 ? 0 : i], r[u][NA == 1 ? 0 : i], h[i], x[u][i]);
-        const bool in = l.live && (decltype(FULL)::value || k < l.len);
-        if (in) {
-          store_vec<T, V>(h0 + (int64_t)k * dh, h);
-        } else if (!decltype(FULL)::value && l.live && k < a.T) {
-          const float zero[V] = {};
-          store_vec<T, V>(pad + (int64_t)k * a.ht, zero);
-        }
-      }
-    };
-    if (full && !cut) walk(std::false_type{}, std::true_type{}); else walk(std::true_type{}, std::false_type{});
+  float q[kScanU][NA], sum[NA] = {}, h[V];
+  bool cut = false;
+  if (!none) {
+    scan_load<T, V>(rx, scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c), dx, k0, l.len, full);
+    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c), da, k0, l.len, full);
   }
-  if (l.live) scan_clear<T, V>(pad, a.ht, stop, end);
-  if (a.final && end == a.T && l.live) store_vec<float, V>(a.final + l.ch, h);
+  // the run from zero; the steps themselves afterwards, with the same code
+  auto walk = [&](auto CUT, auto FULL, auto&& each) {
+#pragma unroll
+    for (int u = 0; u < kScanU; ++u) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float g = q[u][NA == 1 ? 0 : i], x = decltype(FULL)::value || k0 + u < l.len ? rx[u][i] : 0.f;
+        h[i] = gate_apply<decltype(CUT)::value>(g, gate_keeps(g), h[i], x);
+      }
+      each(u);
+    }
+  };
+  const bool plain = full && !cut;
+#pragma unroll
+  for (int i = 0; i < V; ++i) h[i] = 0.f;
+  if (plain) walk(std::false_type{}, std::true_type{}, [](int) {});
+  else if (!none) walk(std::true_type{}, std::false_type{}, [](int) {});
+  float chunk_q, chunk_l;
+  scan_leave<V, NA, false>(meet, a, l, chunk, sum, h, chunk_q, chunk_l);
+  scan_take<V, NA>(meet, a, l, chunk, chunk_q, chunk_l, a.initial);
+  scan_forget<NA>(q);
+#pragma unroll
+  for (int u = 0; u < kScanU; ++u) scan_forget(rx[u]);
+  if (k0 >= a.T) return;
+  scan_own_state<V, NA, false>(h, meet);
+  if (a.state && l.live) store_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch, h);
+  T* h0 = scan_origin(static_cast<T*>(a.h), a, l, a.ht, a.hb, l.c) + (int64_t)k0 * dh;
+  T* pad = static_cast<T*>(a.h) + (int64_t)l.b * a.hb + l.c + (int64_t)k0 * a.ht;        // steps behind the length lie at their own index
+  if (plain) {
+    walk(std::false_type{}, std::true_type{}, [&](int) {
+      if (l.live) store_vec<T, V>(h0, h);
+      scan_next(h0, dh);
+    });
+  } else if (none) {
+    const float zero[V] = {};
+    for (int u = 0; u < kScanU && k0 + u < a.T; ++u, pad += a.ht)
+      if (l.live) store_vec<T, V>(pad, zero);
+  } else {
+    walk(std::true_type{}, std::false_type{}, [&](int u) {
+      const float zero[V] = {};
+      if (l.live && k0 + u < l.len) store_vec<T, V>(h0, h);
+      else if (l.live && k0 + u < a.T) store_vec<T, V>(pad, zero);
+      scan_next(h0, dh);
+      scan_next(pad, a.ht);
+    });
+  }
+  if (a.final && k0 + kScanU >= a.T && l.live) store_vec<float, V>(a.final + l.ch, h);
 }
 
-// The sum over a gate's lanes of this wave, in the lane `at` = 0.  A power of two of them lies on its own boundary.
-__device__ __forceinline__ float gate_lanes_sum(float v, int at, int lanes) {
+// The sums of N values over a gate's lanes of this wave, in the lane `at` = 0.  A power of two of them lies on its own boundary.
+template <int N>
+__device__ __forceinline__ void gate_lanes_sum(float (&v)[N], int at, int lanes) {
+  auto all = [&](auto L) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = lanes_sum<decltype(L)::value>(v[k]);
+  };
   switch (lanes) {
-    case 1: return v;
-    case 2: return lanes_sum<2>(v);
-    case 4: return lanes_sum<4>(v);
-    case 8: return lanes_sum<8>(v);
-    case 16: return lanes_sum<16>(v);
-    case 32: return lanes_sum<32>(v);
-    case 64: return lanes_sum<64>(v);
+    case 1: return;
+    case 2: return all(std::integral_constant<int, 2>{});
+    case 4: return all(std::integral_constant<int, 4>{});
+    case 8: return all(std::integral_constant<int, 8>{});
+    case 16: return all(std::integral_constant<int, 16>{});
+    case 32: return all(std::integral_constant<int, 32>{});
+    case 64: return all(std::integral_constant<int, 64>{});
     default: break;
   }
   int off = 1;
   while (off * 2 < lanes) off *= 2;
   for (; off > 0; off /= 2) {
-    const float other = __shfl_down(v, off, 64);
-    if (at + off < lanes) v += other;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float other = __shfl_down(v[k], off, 64);
+      if (at + off < lanes) v[k] += other;
+    }
   }
-  return v;
 }
 
-// the first launch of a backward in chunks: the runs of all of them but the first.  l = what comes out in front of the run for nothing
-// coming in behind it
-template <typename T, typename TA, int V, int NA>
-__global__ __launch_bounds__(64 * kScanW) void gated_scan_bwd_runs_kernel(const ScanArgs a) {
-  const int wave = threadIdx.x >> 6, chunk = a.chunks - 1 - blockIdx.y;
-  const ScanLane l = scan_lane<V, false>(a);
-  const int64_t dd = a.reverse ? -a.dht : a.dht, da = a.reverse ? -a.at : a.at;
-  const T* d0 = scan_origin(static_cast<const T*>(a.dh), a, l, a.dht, a.dhb, l.c);
-  const TA* a0 = scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c);
-  const int begin = (chunk * kScanW + wave) * a.steps, end = min(begin + a.steps, a.T);
-  float sum[NA] = {}, run[V] = {};
-  reg_vec<T, V> rd[kScanU];
-  reg_vec<TA, NA> ra[kScanU];
-  auto fetch = [&](int k0) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    if (a.dh) scan_load<T, V>(rd, d0, dd, k0, l.len, full);
-    scan_load<TA, NA>(ra, a0, da, k0, l.len, full);
-  };
-  const int stop = scan_stop(l, begin, end), last = stop > begin ? begin + (stop - begin - 1) / kScanU * kScanU : begin - kScanU;
-  if (last >= begin) fetch(last);
-  for (int k0 = last; k0 >= begin; k0 -= kScanU) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    float d[kScanU][V], q[kScanU][NA], r[kScanU][NA];
-    scan_values<T, V>(d, rd, k0, a.dh ? l.len : 0, full && a.dh);
-    const bool cut = scan_gates<TA, NA>(q, r, ra, k0, l.len, full);
-    scan_sum<TA, NA>(sum, q, ra, k0, l.len, full);
-    if (k0 > begin) fetch(k0 - kScanU);
-    auto walk = [&](auto CUT) {
+// ROW: the sums of 16 values over a gate's lanes (a multiple of 16), lane u of a row ending with the u-th.  In four steps a lane and its mirror
+// image in the row, in half of it, and so on each keep one half of the values and give the other away.
+__device__ __forceinline__ float gate_row_sums(const float (&v)[16], int lanes) {
+  const int lane = threadIdx.x & 15;
+  float a[8], b[4], c[2];
 #pragma unroll
-      for (int u = kScanU - 1; u >= 0; --u)
+  for (int k = 0; k < 8; ++k) a[k] = (lane & 8 ? v[k + 8] : v[k]) + dpp_move<0x140>(lane & 8 ? v[k] : v[k + 8]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) run[i] = gate_times<decltype(CUT)::value>(q[u][NA == 1 ? 0 : i], r[u][NA == 1 ? 0 : i], run[i] + d[u][i]);
-    };
-    if (cut) walk(std::true_type{}); else walk(std::false_type{});
-  }
-  scan_runs<V, NA>(a, l, chunk, sum, run, true);
+  for (int k = 0; k < 4; ++k) b[k] = (lane & 4 ? a[k + 4] : a[k]) + dpp_move<0x141>(lane & 4 ? a[k] : a[k + 4]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) c[k] = (lane & 2 ? b[k + 2] : b[k]) + dpp_move<0x1B>(lane & 2 ? b[k] : b[k + 2]);
+  float s = (lane & 1 ? c[1] : c[0]) + dpp_move<0xB1>(lane & 1 ? c[0] : c[1]);
+  // the rows of a gate, in order: the first one of each gate ends with the sum
+  const float s1 = __shfl_down(s, 16, 64), s2 = __shfl_down(s, 32, 64), s3 = __shfl_down(s, 48, 64);
+  if (lanes > 16) s += s1;
+  if (lanes > 32) s += s2;
+  if (lanes > 48) s += s3;
+  return s;
 }
 
-// GROUPED: a gate has several channels (NA = 1); otherwise every channel has its own (NA = V).
-template <typename T, typename TA, int V, int NA, bool GROUPED>
-__global__ __launch_bounds__(64 * kScanW) void gated_scan_bwd_kernel(const ScanArgs a) {
-  const int wave = threadIdx.x >> 6, chunk = blockIdx.y;
-  const ScanLane l = scan_lane<V, GROUPED>(a);
+// GROUPED: a gate has several channels (NA = 1); otherwise every channel has its own (NA = V).  Chunks are counted from the end.
+// 8 bytes a lane and step need 180 to 250 registers, 2 waves a SIMD (3 of them, spilling: 131 -> 163 us); less fits 128 with a
+// step's a_k h_{k-1} kept for half of the steps at a time.
+template <typename T, typename TA, int V, int NA, bool GROUPED, bool ROW>
+__global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated_scan_bwd_kernel(const ScanArgs a) {
+  __shared__ ScanMeet<V, NA> meet;
+  const uint32_t number = scan_ticket(a, meet);
+  const int wave = threadIdx.x >> 6, chunk = number / a.blocks;
+  const ScanLane l = scan_lane<V, GROUPED>(a, number % a.blocks);
   const int64_t C = (int64_t)a.B * a.D;
   const int64_t dx = a.reverse ? -a.xt : a.xt, da = a.reverse ? -a.at : a.at, dd = a.reverse ? -a.dht : a.dht;
   const int64_t ddx = a.reverse ? -a.dxt : a.dxt, dda = a.reverse ? -a.dat : a.dat;
   const int gate = NA == 1 ? l.gate : l.c;
-  const T* x0 = scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c);
-  const T* d0 = scan_origin(static_cast<const T*>(a.dh), a, l, a.dht, a.dhb, l.c);
-  const TA* a0 = scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, gate);
-  T* gx0 = scan_origin(static_cast<T*>(a.dx), a, l, a.dxt, a.dxb, l.c);
-  T* padx = static_cast<T*>(a.dx) + (int64_t)l.b * a.dxb + l.c;
-  TA* ga0 = scan_origin(static_cast<TA*>(a.dalpha), a, l, a.dat, a.dab, gate);
-  TA* pada = static_cast<TA*>(a.dalpha) + (int64_t)l.b * a.dab + gate;
-  const int segs = GROUPED ? (a.D / a.G / V + 63) / 64 : 1;
-  const int begin = (chunk * kScanW + wave) * a.steps, end = min(begin + a.steps, a.T);
-  if (begin >= end) return;
-  const int stop = scan_stop(l, begin, end), last = stop > begin ? begin + (stop - begin - 1) / kScanU * kScanU : begin - kScanU;
+  const int k0 = ((a.chunks - 1 - chunk) * kScanW + wave) * kScanU;
+  const bool full = __all(k0 + kScanU <= l.len), none = !__any(l.live && k0 < l.len), begun = k0 < a.T;
   reg_vec<T, V> rx[kScanU], rd[kScanU];
-  reg_vec<TA, NA> ra[kScanU];
   reg_vec<float, V> rs;
-  auto fetch = [&](int k0) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    scan_load<T, V>(rx, x0, dx, k0, l.len, full);
-    if (a.dh) scan_load<T, V>(rd, d0, dd, k0, l.len, full);
-    scan_load<TA, NA>(ra, a0, da, k0, l.len, full);
-    rs = load_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch);
-  };
-  if (last >= begin) fetch(last);
-  float g[V];
+  float q[kScanU][NA], sum[NA] = {}, g[V];
+  bool cut = false;
 #pragma unroll
-  for (int i = 0; i < V; ++i) g[i] = a.dfinal && l.live ? a.dfinal[l.ch + i] : 0.f;
-  if (end < a.T) scan_compose<V>(g, a, l.ch, chunk, wave, a.chunks - 1, kScanW - 1);
-  for (int k0 = last; k0 >= begin; k0 -= kScanU) {
-    const bool full = __all(k0 + kScanU <= l.len);
-    float x[kScanU][V], d[kScanU][V], q[kScanU][NA], r[kScanU][NA], h[V];
-    scan_values<T, V>(x, rx, k0, l.len, full);
-    scan_values<T, V>(d, rd, k0, a.dh ? l.len : 0, full && a.dh);
-    const bool cut = scan_gates<TA, NA>(q, r, ra, k0, l.len, full);
+  for (int u = 0; u < kScanU; ++u) rd[u] = reg_vec<T, V>{};
+  if (!none) {
+    if (a.dh) scan_load<T, V>(rd, scan_origin(static_cast<const T*>(a.dh), a, l, a.dht, a.dhb, l.c), dd, k0, l.len, full);
+    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, gate), da, k0, l.len, full);
+  }
+  const bool plain = full && !cut;
+  auto value = [&](const reg_vec<T, V>& r, int u, int i, bool all) { return all || k0 + u < l.len ? r[i] : 0.f; };
+  auto back = [&](auto CUT, auto FULL) {
+#pragma unroll
+    for (int u = kScanU - 1; u >= 0; --u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float c = q[u][NA == 1 ? 0 : i], d = value(rd[u], u, i, decltype(FULL)::value);
+        g[i] = gate_times<decltype(CUT)::value>(c, gate_keeps(c), g[i] + d);
+      }
+  };
+#pragma unroll
+  for (int i = 0; i < V; ++i) g[i] = 0.f;
+  if (plain) back(std::false_type{}, std::true_type{});
+  else if (!none) back(std::true_type{}, std::false_type{});
+  float chunk_q, chunk_l;
+  scan_leave<V, NA, true>(meet, a, l, chunk, sum, g, chunk_q, chunk_l);
+  // (x and the state are needed from here on: their way from memory is the wait for the other chunks)
+  if (!none) scan_load<T, V>(rx, scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c), dx, k0, l.len, full);
+  if (begun) rs = load_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch);
+  scan_take<V, NA>(meet, a, l, chunk, chunk_q, chunk_l, a.dfinal);
+  scan_forget<NA>(q);
+#pragma unroll
+  for (int u = 0; u < kScanU; ++u) scan_forget(rd[u]);
+  if (!begun) return;
+  scan_own_state<V, NA, true>(g, meet);
+  const int segs = GROUPED ? (a.D / a.G / V + 63) / 64 : 1;
+  TA* const alpha0 = scan_origin(static_cast<TA*>(a.dalpha), a, l, a.dat, a.dab, gate);
+  TA* const alpha_pad = static_cast<TA*>(a.dalpha) + (int64_t)l.b * a.dab + gate;
+  // the gradient of the gate of step k, where the row has it
+  auto put_gate = [&](int k, float v) {
+    if (!l.live || k >= a.T) return;
+    const bool in = k < l.len;
+    if (segs > 1) a.part[((int64_t)(in && a.reverse ? l.len - 1 - k : k) * a.B * a.G + l.group) * segs + l.seg] = v;
+    else if (in) alpha0[(int64_t)k * dda] = (TA)v;
+    else alpha_pad[(int64_t)k * a.dat] = (TA)v;
+  };
+  if (none) {
+    const float zero[V] = {}, none_of[NA] = {};
+    T* padx = static_cast<T*>(a.dx) + (int64_t)l.b * a.dxb + l.c;
+    for (int k = k0; k < k0 + kScanU && k < a.T; ++k) {
+      if (l.live) store_vec<T, V>(padx + (int64_t)k * a.dxt, zero);
+      if constexpr (GROUPED) {
+        if (l.first) put_gate(k, 0.f);
+      } else {
+        if (l.live) store_vec<TA, NA>(alpha_pad + (int64_t)k * a.dat, none_of);
+      }
+    }
+    if (a.dinitial && k0 == 0 && l.live) store_vec<float, V>(a.dinitial + l.ch, g);
+    return;
+  }
+  T* gx0 = scan_origin(static_cast<T*>(a.dx), a, l, a.dxt, a.dxb, l.c) + (int64_t)(k0 + kScanU - 1) * ddx;
+  T* padx = static_cast<T*>(a.dx) + (int64_t)l.b * a.dxb + l.c + (int64_t)(k0 + kScanU - 1) * a.dxt;
+  TA* ga0 = alpha0 + (int64_t)(k0 + kScanU - 1) * dda;
+  TA* pada = alpha_pad + (int64_t)(k0 + kScanU - 1) * a.dat;
+  float gate_grad[GROUPED ? kScanU : 1];
+  auto walk = [&](auto CUT, auto FULL) {
+    constexpr bool cuts = decltype(CUT)::value, all = decltype(FULL)::value;
+    // (the later half first: the walk to it passes the earlier one)
+    constexpr int HALF = sizeof(T) * V == 8 ? kScanU : kScanU / 2;
+#pragma unroll
+    for (int part = kScanU / HALF - 1; part >= 0; --part) {
+    float p[HALF][V], h[V];              // p: a_k h_{k-1}
+    if (part == 0 && HALF < kScanU) {
+      scan_forget<NA>(q);
+#pragma unroll
+      for (int u = 0; u < HALF; ++u) scan_forget(rx[u]);
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) h[i] = rs[i];
-    if (k0 > begin) fetch(k0 - kScanU);
-    auto walk = [&](auto CUT, auto FULL) {
-      constexpr bool cuts = decltype(CUT)::value, all = decltype(FULL)::value;
-      // x becomes a_k h_{k-1}
 #pragma unroll
-      for (int u = 0; u < kScanU; ++u)
+    for (int u = 0; u < (part + 1) * HALF; ++u)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float p = gate_times<cuts>(q[u][NA == 1 ? 0 : i], r[u][NA == 1 ? 0 : i], h[i]);
-          h[i] = p + x[u][i];
-          x[u][i] = p;
-        }
+      for (int i = 0; i < V; ++i) {
+        const float c = q[u][NA == 1 ? 0 : i], before = gate_times<cuts>(c, gate_keeps(c), h[i]);
+        if (u >= part * HALF) p[u - part * HALF][i] = before;
+        h[i] = before + value(rx[u], u, i, all);
+      }
 #pragma unroll
-      for (int u = kScanU - 1; u >= 0; --u) {
-        const int k = k0 + u;
-        float gx[V], galpha[NA] = {};
+    for (int u = (part + 1) * HALF - 1; u >= part * HALF; --u) {
+      const int k = k0 + u;
+      const bool in = l.live && (all || k < l.len), behind = !all && l.live && !in && k < a.T;
+      float gx[V], galpha[NA] = {};
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          gx[i] = g[i] + d[u][i];
-          galpha[NA == 1 ? 0 : i] += x[u][i] * gx[i];
-          g[i] = gate_times<cuts>(q[u][NA == 1 ? 0 : i], r[u][NA == 1 ? 0 : i], gx[i]);
-        }
-        const bool in = l.live && (all || k < l.len), behind = !all && l.live && !in && k < a.T;
+      for (int i = 0; i < V; ++i) {
+        const float c = q[u][NA == 1 ? 0 : i];
+        gx[i] = g[i] + value(rd[u], u, i, all);
+        galpha[NA == 1 ? 0 : i] += p[u - part * HALF][i] * gx[i];
+        g[i] = gate_times<cuts>(c, gate_keeps(c), gx[i]);
+      }
+      if (in) {
+        store_vec<T, V>(gx0, gx);
+      } else if (behind) {
+        const float zero[V] = {};
+        store_vec<T, V>(padx, zero);
+      }
+      scan_next(gx0, -ddx);
+      if constexpr (!all) scan_next(padx, -a.dxt);
+      if constexpr (GROUPED) {
+        gate_grad[u] = in ? galpha[0] : 0.f;
+      } else {
         if (in) {
-          store_vec<T, V>(gx0 + (int64_t)k * ddx, gx);
-        } else if (behind) {
-          const float zero[V] = {};
-          store_vec<T, V>(padx + (int64_t)k * a.dxt, zero);
-        }
-        if constexpr (GROUPED) {
-          const float out[1] = {gate_lanes_sum(in ? galpha[0] : 0.f, l.at, l.lanes)};
-          if (l.first && segs > 1) {
-            const int64_t t = in && a.reverse ? l.len - 1 - k : k;
-            if (in || behind) a.part[(t * a.B * a.G + l.group) * segs + l.seg] = out[0];
-          } else if (l.first && in) {
-            store_vec<TA, 1>(ga0 + (int64_t)k * dda, out);
-          } else if (l.first && behind) {
-            store_vec<TA, 1>(pada + (int64_t)k * a.dat, out);
-          }
-        } else if (in) {
-          store_vec<TA, NA>(ga0 + (int64_t)k * dda, galpha);
+          store_vec<TA, NA>(ga0, galpha);
         } else if (behind) {
           const float zero[NA] = {};
-          store_vec<TA, NA>(pada + (int64_t)k * a.dat, zero);
+          store_vec<TA, NA>(pada, zero);
         }
+        scan_next(ga0, -dda);
+        if constexpr (!all) scan_next(pada, -a.dat);
       }
-    };
-    if (full && !cut) walk(std::false_type{}, std::true_type{}); else walk(std::true_type{}, std::false_type{});
-  }
-  if (l.live && stop < end) {
-    scan_clear<T, V>(padx, a.dxt, stop, end);
-    if constexpr (!GROUPED) {
-      scan_clear<TA, NA>(pada, a.dat, stop, end);
-    } else if (l.first) {
-      if (segs > 1)
-        scan_clear<float, 1>(a.part + l.group * segs + l.seg, (int64_t)a.B * a.G * segs, stop, end);
-      else
-        scan_clear<TA, 1>(pada, a.dat, stop, end);
+    }
+    }
+  };
+  if (plain) walk(std::false_type{}, std::true_type{}); else walk(std::true_type{}, std::false_type{});
+  if constexpr (ROW) {
+    const float v = gate_row_sums(gate_grad, l.lanes);
+    if (l.at < 16) put_gate(k0 + (threadIdx.x & 15), v);
+  } else if constexpr (GROUPED) {
+    gate_lanes_sum<kScanU>(gate_grad, l.at, l.lanes);
+    if (l.first) {
+#pragma unroll
+      for (int u = 0; u < kScanU; ++u) put_gate(k0 + u, gate_grad[u]);
     }
   }
-  if (a.dinitial && begin == 0 && l.live) store_vec<float, V>(a.dinitial + l.ch, g);
+  if (a.dinitial && k0 == 0 && l.live) store_vec<float, V>(a.dinitial + l.ch, g);
 }
 
 // adds the waves' partial sums of gates wider than a wave
@@ -543,21 +685,19 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const T* __restric
   const int64_t b = i / D;
   const int c = (int)(i - b * D);
   float* s = state + b * sb + c;
-  const float v = gate_apply(gate_of((float)alpha[b * ab + c / per]), *s, (float)x[b * xb + c]);
+  const float q = gate_of((float)alpha[b * ab + c / per]), v = gate_apply<true>(q, gate_keeps(q), *s, (float)x[b * xb + c]);
   *s = v;
   h[i] = (T)v;
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------
 struct ScanPlan {
-  int V, steps, chunks, segs;
-  int64_t fwd_blocks, bwd_blocks;
+  int V, chunks, segs;
+  int64_t fwd_blocks, bwd_blocks, words;      // words: 64-bit words of workspace for the chunks, the ticket's included
 };
 
-// V channels a lane: up to 8 bytes of x and of gates of their own a step, where they divide the channels of a row (of a gate).  Runs: as
-// many as give 2048 waves, two for every SIMD -- at (4096, 8, 2048) bf16 forward and backward took 375 us with 1024 waves, 285 with 1536,
-// 238 with 2048, 297 with 3072, 254 with 4096: an uneven number leaves a tail, more of them read more runs -- of U steps at least, and 64
-// workgroups of them along time at most, since every wave composes those in front of its own.
+// V channels a lane: up to 8 bytes of x and of gates of their own a step, where they divide the channels of a row (of a gate): for bf16
+// (4096, 8, 2048), 32 decays, 216 us forward and backward with 4 or 2 channels and 286 with 1.
 static ScanPlan scan_plan(const socmx_scan& s) {
   ScanPlan p;
   const int64_t C = (int64_t)s.B * s.D;
@@ -566,8 +706,7 @@ static ScanPlan scan_plan(const socmx_scan& s) {
   const int bytes = (s.type == SOCMX_F32 ? 4 : 2) + (per > 1 ? 0 : s.gate_type == SOCMX_F32 ? 4 : 2);
   for (int v = 4; v > 1; v /= 2)
     if (bytes * v <= 8 && s.D % v == 0 && (per == 1 || per % v == 0)) { p.V = v; break; }
-  const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V);
-  p.fwd_blocks = p.bwd_blocks = groups;
+  p.fwd_blocks = p.bwd_blocks = (C + 64 * p.V - 1) / (64 * p.V);
   p.segs = 1;
   if (per > 1) {
     const int wide = per / p.V;
@@ -575,10 +714,8 @@ static ScanPlan scan_plan(const socmx_scan& s) {
     const int64_t gates = (int64_t)s.B * s.G;
     p.bwd_blocks = wide <= 64 ? (gates + 64 / wide - 1) / (64 / wide) : gates * p.segs;
   }
-  const int64_t runs = std::max<int64_t>(1, std::min<int64_t>(2048 / groups, 64 * kScanW));
-  const int64_t steps = std::max<int64_t>(kScanU, ((s.T + runs - 1) / runs + kScanU - 1) / kScanU * kScanU);
-  p.steps = (int)steps;
-  p.chunks = (int)((s.T + steps * kScanW - 1) / (steps * kScanW));
+  p.chunks = (s.T + kScanTile - 1) / kScanTile;
+  p.words = p.chunks > 1 ? p.chunks * C + ((p.chunks + kGroup - 1) / kGroup * C + 1) / 2 + 1 : 0;
   return p;
 }
 
@@ -595,55 +732,60 @@ static ScanArgs scan_args(const socmx_scan& s, const ScanPlan& p) {
   a.lengths = s.lengths;
   a.xt = s.x_stride_t; a.xb = s.x_stride_b; a.at = s.gate_stride_t; a.ab = s.gate_stride_b;
   a.T = s.T; a.B = s.B; a.D = s.D; a.G = s.G; a.reverse = s.reverse != 0;
-  a.steps = p.steps; a.chunks = p.chunks;
+  a.chunks = p.chunks;
   return a;
 }
 
-// (runs are needed wherever a wave begins behind step 0, also inside the one workgroup of a short scan)
-static inline bool scan_has_runs(const ScanPlan& p, int T) { return p.steps < T; }
-
 template <typename T, typename TA, int V, bool BWD>
-static int launch_scan(const ScanArgs& a, const ScanPlan& p, void* stream) {
-  const bool own = a.G == a.D;
-  const dim3 block(64 * kScanW), runs((unsigned)p.fwd_blocks, p.chunks), grid((unsigned)(BWD ? p.bwd_blocks : p.fwd_blocks), p.chunks);
-  int err = 0;
+static int launch_scan(ScanArgs a, const ScanPlan& p, void* workspace, void* stream) {
+  const bool own = a.G == a.D, row = !own && a.D / a.G % (16 * V) == 0;      // (whole rows of lanes share a gate)
+  const int64_t blocks = BWD ? p.bwd_blocks : p.fwd_blocks;
+  a.blocks = (uint32_t)blocks;
+  if (p.chunks > 1) {
+    const int64_t C = (int64_t)a.B * a.D;
+    a.word = static_cast<uint64_t*>(workspace);
+    a.mark = reinterpret_cast<float*>(a.word + p.chunks * C);
+    a.ticket = reinterpret_cast<uint32_t*>(a.word + p.words - 1);
+    if (const int err = launch(gated_scan_clear_kernel, dim3((unsigned)((p.words - 1 + 255) / 256)), dim3(256), 0, stream, a.word, p.words - 1, a.ticket))
+      return err;
+  }
+  const dim3 grid((unsigned)(blocks * p.chunks)), block(64 * kScanW);
+  int err = SOCMX_E_DIM;               // (the forms that scan_plan never asks for are not compiled)
+  constexpr bool can_own = (sizeof(T) + sizeof(TA)) * V <= 8, can_share = sizeof(T) * V <= 8;
   if constexpr (!BWD) {
-    if (scan_has_runs(p, a.T))
-      err = own ? launch(gated_scan_fwd_runs_kernel<T, TA, V, V>, runs, block, 0, stream, a)
-                : launch(gated_scan_fwd_runs_kernel<T, TA, V, 1>, runs, block, 0, stream, a);
-    if (err) return err;
-    return own ? launch(gated_scan_fwd_kernel<T, TA, V, V>, grid, block, 0, stream, a)
-               : launch(gated_scan_fwd_kernel<T, TA, V, 1>, grid, block, 0, stream, a);
+    if constexpr (can_own)
+      if (own) return launch(gated_scan_fwd_kernel<T, TA, V, V, false>, grid, block, 0, stream, a);
+    if constexpr (can_share)
+      if (!own)
+        return row ? launch(gated_scan_fwd_kernel<T, TA, V, 1, true>, grid, block, 0, stream, a)
+                   : launch(gated_scan_fwd_kernel<T, TA, V, 1, false>, grid, block, 0, stream, a);
+    return err;
   } else {
-    if (scan_has_runs(p, a.T))
-      err = own ? launch(gated_scan_bwd_runs_kernel<T, TA, V, V>, runs, block, 0, stream, a)
-                : launch(gated_scan_bwd_runs_kernel<T, TA, V, 1>, runs, block, 0, stream, a);
-    if (err) return err;
-    err = own ? launch(gated_scan_bwd_kernel<T, TA, V, V, false>, grid, block, 0, stream, a)
-              : launch(gated_scan_bwd_kernel<T, TA, V, 1, true>, grid, block, 0, stream, a);
+    if constexpr (can_own)
+      if (own) err = launch(gated_scan_bwd_kernel<T, TA, V, V, false, false>, grid, block, 0, stream, a);
+    if constexpr (can_share)
+      if (!own)
+        err = row ? launch(gated_scan_bwd_kernel<T, TA, V, 1, true, true>, grid, block, 0, stream, a)
+                  : launch(gated_scan_bwd_kernel<T, TA, V, 1, true, false>, grid, block, 0, stream, a);
     if (err || p.segs == 1) return err;
     const int64_t sums = (int64_t)a.T * a.B * a.G;
     return launch(gated_scan_bwd_finish_kernel<TA>, dim3((unsigned)((sums + 255) / 256)), dim3(256), 0, stream, a, p.segs);
   }
 }
 
-static inline int64_t scan_run_floats(const socmx_scan& s, const ScanPlan& p) {
-  return scan_has_runs(p, s.T) ? (int64_t)p.chunks * (1 + kScanW) * 2 * s.B * s.D : 0;
-}
-
 template <typename T, typename TA, bool BWD>
-static int launch_scan_v(const ScanArgs& a, const ScanPlan& p, void* stream) {
-  if (p.V == 4) return launch_scan<T, TA, 4, BWD>(a, p, stream);
-  if (p.V == 2) return launch_scan<T, TA, 2, BWD>(a, p, stream);
-  return launch_scan<T, TA, 1, BWD>(a, p, stream);
+static int launch_scan_v(const ScanArgs& a, const ScanPlan& p, void* ws, void* stream) {
+  if (p.V == 4) return launch_scan<T, TA, 4, BWD>(a, p, ws, stream);
+  if (p.V == 2) return launch_scan<T, TA, 2, BWD>(a, p, ws, stream);
+  return launch_scan<T, TA, 1, BWD>(a, p, ws, stream);
 }
 
 template <bool BWD>
-static int dispatch_scan(const socmx_scan& s, const ScanArgs& a, const ScanPlan& p, void* stream) {
+static int dispatch_scan(const socmx_scan& s, const ScanArgs& a, const ScanPlan& p, void* ws, void* stream) {
   const bool wide = s.gate_type == SOCMX_F32;
-  if (s.type == SOCMX_F32) return launch_scan_v<float, float, BWD>(a, p, stream);
-  if (s.type == SOCMX_BF16) return wide ? launch_scan_v<bf16_t, float, BWD>(a, p, stream) : launch_scan_v<bf16_t, bf16_t, BWD>(a, p, stream);
-  return wide ? launch_scan_v<f16_t, float, BWD>(a, p, stream) : launch_scan_v<f16_t, f16_t, BWD>(a, p, stream);
+  if (s.type == SOCMX_F32) return launch_scan_v<float, float, BWD>(a, p, ws, stream);
+  if (s.type == SOCMX_BF16) return wide ? launch_scan_v<bf16_t, float, BWD>(a, p, ws, stream) : launch_scan_v<bf16_t, bf16_t, BWD>(a, p, ws, stream);
+  return wide ? launch_scan_v<f16_t, float, BWD>(a, p, ws, stream) : launch_scan_v<f16_t, f16_t, BWD>(a, p, ws, stream);
 }
 
 }  // namespace socmx
@@ -655,10 +797,11 @@ extern "C" int socmx_gated_scan_sizes(const socmx_scan* scan, int64_t* state_flo
   if (const int bad = scan_check(scan)) return bad;
   if (!state_floats || !fwd_workspace_floats || !bwd_workspace_floats) return SOCMX_E_NULL;
   const ScanPlan p = scan_plan(*scan);
-  const int64_t C = (int64_t)scan->B * scan->D, runs = scan_run_floats(*scan, p);
+  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  const int64_t C = (int64_t)scan->B * scan->D;
   *state_floats = (scan->T + kScanU - 1) / kScanU * C;
-  *fwd_workspace_floats = runs;
-  *bwd_workspace_floats = runs + (p.segs > 1 ? (int64_t)scan->T * scan->B * scan->G * p.segs : 0);
+  *fwd_workspace_floats = 2 * p.words;
+  *bwd_workspace_floats = 2 * p.words + (p.segs > 1 ? (int64_t)scan->T * scan->B * scan->G * p.segs : 0);
   return 0;
 }
 
@@ -668,11 +811,12 @@ extern "C" int socmx_gated_scan_fwd(const socmx_scan* scan, const void* x, const
   if (const int bad = scan_check(scan)) return bad;
   if (!x || !log_decay || !h) return SOCMX_E_NULL;
   const ScanPlan p = scan_plan(*scan);
-  if (scan_has_runs(p, scan->T) && !workspace) return SOCMX_E_WORKSPACE;
+  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  if (p.chunks > 1 && (!workspace || (uintptr_t)workspace % 8)) return SOCMX_E_WORKSPACE;
   ScanArgs a = scan_args(*scan, p);
   a.x = x; a.alpha = log_decay; a.initial = initial; a.h = h; a.ht = h_stride_t; a.hb = h_stride_b;
-  a.final = final_state; a.state = states; a.run = workspace;
-  return dispatch_scan<false>(*scan, a, p, stream);
+  a.final = final_state; a.state = states;
+  return dispatch_scan<false>(*scan, a, p, workspace, stream);
 }
 
 extern "C" int socmx_gated_scan_bwd(const socmx_scan* scan, const void* x, const void* log_decay, const float* states, const void* dh,
@@ -682,14 +826,14 @@ extern "C" int socmx_gated_scan_bwd(const socmx_scan* scan, const void* x, const
   if (const int bad = scan_check(scan)) return bad;
   if (!x || !log_decay || !states || !dx || !dlog_decay) return SOCMX_E_NULL;
   const ScanPlan p = scan_plan(*scan);
-  if ((scan_has_runs(p, scan->T) || p.segs > 1) && !workspace) return SOCMX_E_WORKSPACE;
+  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  if ((p.chunks > 1 || p.segs > 1) && (!workspace || (uintptr_t)workspace % 8)) return SOCMX_E_WORKSPACE;
   ScanArgs a = scan_args(*scan, p);
   a.x = x; a.alpha = log_decay; a.state = const_cast<float*>(states); a.dh = dh; a.dht = dh_stride_t; a.dhb = dh_stride_b;
   a.dfinal = dfinal; a.dx = dx; a.dxt = dx_stride_t; a.dxb = dx_stride_b;
   a.dalpha = dlog_decay; a.dat = dgate_stride_t; a.dab = dgate_stride_b; a.dinitial = dinitial;
-  a.run = workspace;
-  a.part = workspace ? workspace + scan_run_floats(*scan, p) : nullptr;
-  return dispatch_scan<true>(*scan, a, p, stream);
+  a.part = workspace ? workspace + 2 * p.words : nullptr;
+  return dispatch_scan<true>(*scan, a, p, workspace, stream);
 }
 
 extern "C" int socmx_gated_scan_step(int32_t type, int32_t gate_type, int32_t B, int32_t D, int32_t G, const void* x, int64_t x_stride,

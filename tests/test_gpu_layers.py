@@ -367,6 +367,50 @@ def test_gated_scan_forgets_at_a_decay_of_zero():
     assert bool((gx[:128] == 0).all()) and bool((ga[cut] == 0).all()) and bool(torch.isfinite(ga[129:]).all())
 
 
+@pytest.mark.parametrize("kind,gkind", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("T,D,G", [(40, 96, 3), (150, 192, 3), (129, 192, 2), (33, 128, 1), (300, 320, 2), (20, 1280, 1), (140, 768, 4)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_gated_scan_shared_gates_in_whole_rows_of_lanes(kind, gkind, T, D, G, reverse):
+    lengths = [T, 0, 17, T - 1, 1]
+    x, a, initial, dh, dfinal = scan_case(T, len(lengths), D, G, T + D + G, kind, gkind, resets=0.01)
+    scan_check(x.to(DEV), a.to(DEV), initial, dh.to(DEV), dfinal, lengths=lengths, reverse=reverse)
+
+
+def test_gated_scan_forgets_behind_any_decay():
+    """Infinite and NaN decays in front of a cut, in the same run of steps, in another one and far before it, stay in front of it."""
+    T, B, D = 700, 1, 4
+    x, a, initial, _, _ = scan_case(T, B, D, D, 12)
+    cut = [20, 100, 400, 690]
+    a[cut] = -math.inf
+    clean = [t.cpu() for t in layers.gated_scan(x.to(DEV), a.to(DEV), initial.to(DEV))]
+    a[18], a[70], a[140] = math.inf, math.nan, math.inf
+    h, final = (t.cpu() for t in layers.gated_scan(x.to(DEV), a.to(DEV), initial.to(DEV)))
+    for lo, hi in ((0, 18), (20, 70), (100, 140), (400, T)):
+        assert torch.equal(h[lo:hi], clean[0][lo:hi]), (lo, hi)
+    assert torch.equal(final, clean[1])
+    for lo, hi in ((18, 20), (70, 100), (140, 400)):
+        assert not bool(torch.isfinite(h[lo:hi]).any()), (lo, hi)
+
+
+def test_gated_scan_products_of_decays_beyond_float32():
+    """No single decay forgets, but those of a run multiply to less than 2^-126: NaN stays NaN.  They multiply to more than the
+    largest number: a state of zero stays zero, in either direction of the derivative."""
+    T = 900
+    x = torch.zeros(T, 1, 3, device=DEV)
+    x[5, 0, 0] = math.nan
+    h, final = layers.gated_scan(x, torch.full((T, 1, 3), -10.0, device=DEV))
+    assert bool(h[5:, 0, 0].isnan().all()) and bool(final[0, 0].isnan()) and bool((h[..., 1:] == 0).all())
+    a = torch.full((T, 1, 3), 3.0, device=DEV)
+    a[-1] = -math.inf
+    x = torch.zeros(T, 1, 3, device=DEV)
+    x[-1] = 2.0
+    ts = [t.requires_grad_() for t in (x, a)]
+    h, final = layers.gated_scan(*ts)
+    assert bool((h[:-1] == 0).all()) and bool((h[-1] == 2).all())
+    gx, ga = torch.autograd.grad(final.sum(), ts)
+    assert bool((gx[:-1] == 0).all()) and bool((gx[-1] == 1).all()) and bool((ga == 0).all())
+
+
 def test_gated_scan_long_memory_is_exact():
     """A constant decay with a memory of 20000 steps: rounding exp(alpha) to float32 would be off by up to 20000 2^-25 = 6e-4 of the
     steady state; a gate kept as exp(alpha) - 1 leaves one rounding a step, in either direction."""
