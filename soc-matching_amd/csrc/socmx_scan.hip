@@ -27,9 +27,10 @@
 // products are summed across the lanes in a fixed order, gates wider than a wave leave one partial sum a wave for another launch.  No
 // floating-point atomics.
 //
-// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 118 us (4.3 TB/s of x, alpha, h and states) + 172 us (5.0): memory, a copy of
-// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 84 us (3.5 TB/s) + 131 us (3.3); rows that are on average 3/4
-// full 72 + 111, of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 20 + 28.
+// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 116 us (4.4 TB/s of x, alpha, h and states) + 160 us (5.3): memory, a copy of
+// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 80 us (3.6 TB/s) + 126 us (3.4); rows that are on average 3/4
+// full 66 + 100, of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 19 + 23.  Results leave past the caches (121 + 170, 84 + 131,
+// 20 + 28 otherwise).
 // Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57.  U = 16, W = 8 and
 // kGroup = 16 were the best or within 2 % of it among U 4, 8, 16, W 4, 8, 16 and groups of 16, 32; chunks wait for each other 3 to 7 % of the time.
 #include <hip/hip_runtime.h>
@@ -446,18 +447,18 @@ __global__ __launch_bounds__(64 * kScanW, 4) void gated_scan_fwd_kernel(const Sc
   T* pad = static_cast<T*>(a.h) + (int64_t)l.b * a.hb + l.c + (int64_t)k0 * a.ht;        // steps behind the length lie at their own index
   if (plain) {
     walk(std::false_type{}, std::true_type{}, [&](int) {
-      if (l.live) store_vec<T, V>(h0, h);
+      if (l.live) stream_vec<T, V>(h0, h);
       scan_next(h0, dh);
     });
   } else if (none) {
     const float zero[V] = {};
     for (int u = 0; u < kScanU && k0 + u < a.T; ++u, pad += a.ht)
-      if (l.live) store_vec<T, V>(pad, zero);
+      if (l.live) stream_vec<T, V>(pad, zero);
   } else {
     walk(std::true_type{}, std::false_type{}, [&](int u) {
       const float zero[V] = {};
-      if (l.live && k0 + u < l.len) store_vec<T, V>(h0, h);
-      else if (l.live && k0 + u < a.T) store_vec<T, V>(pad, zero);
+      if (l.live && k0 + u < l.len) stream_vec<T, V>(h0, h);
+      else if (l.live && k0 + u < a.T) stream_vec<T, V>(pad, zero);
       scan_next(h0, dh);
       scan_next(pad, a.ht);
     });
@@ -579,11 +580,11 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
     const float zero[V] = {}, none_of[NA] = {};
     T* padx = static_cast<T*>(a.dx) + (int64_t)l.b * a.dxb + l.c;
     for (int k = k0; k < k0 + kScanU && k < a.T; ++k) {
-      if (l.live) store_vec<T, V>(padx + (int64_t)k * a.dxt, zero);
+      if (l.live) stream_vec<T, V>(padx + (int64_t)k * a.dxt, zero);
       if constexpr (GROUPED) {
         if (l.first) put_gate(k, 0.f);
       } else {
-        if (l.live) store_vec<TA, NA>(alpha_pad + (int64_t)k * a.dat, none_of);
+        if (l.live) stream_vec<TA, NA>(alpha_pad + (int64_t)k * a.dat, none_of);
       }
     }
     if (a.dinitial && k0 == 0 && l.live) store_vec<float, V>(a.dinitial + l.ch, g);
@@ -629,10 +630,10 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
         g[i] = gate_times<cuts>(c, gate_keeps(c), gx[i]);
       }
       if (in) {
-        store_vec<T, V>(gx0, gx);
+        stream_vec<T, V>(gx0, gx);
       } else if (behind) {
         const float zero[V] = {};
-        store_vec<T, V>(padx, zero);
+        stream_vec<T, V>(padx, zero);
       }
       scan_next(gx0, -ddx);
       if constexpr (!all) scan_next(padx, -a.dxt);
@@ -640,10 +641,10 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
         gate_grad[u] = in ? galpha[0] : 0.f;
       } else {
         if (in) {
-          store_vec<TA, NA>(ga0, galpha);
+          stream_vec<TA, NA>(ga0, galpha);
         } else if (behind) {
           const float zero[NA] = {};
-          store_vec<TA, NA>(pada, zero);
+          stream_vec<TA, NA>(pada, zero);
         }
         scan_next(ga0, -dda);
         if constexpr (!all) scan_next(pada, -a.dat);

@@ -56,9 +56,9 @@ __device__ __forceinline__ reg_vec<T, N> load_vec(const T* p, int n) {
   return r;
 }
 
-// rounds to T (to nearest, ties to even) and stores
+// rounds to T (to nearest, ties to even)
 template <typename T, int N>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+__device__ __forceinline__ typename mem_vec<T, N>::type round_vec(const float (&x)[N]) {
   typename mem_vec<T, N>::type v;
   if constexpr (N == 1) {
     v = (T)x[0];
@@ -66,7 +66,29 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
   }
-  *reinterpret_cast<typename mem_vec<T, N>::type*>(p) = v;
+  return v;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+  *reinterpret_cast<typename mem_vec<T, N>::type*>(p) = round_vec<T, N>(x);
+}
+
+// for what the kernel writes once and nothing near reads: it takes no cache lines from the loads
+template <typename T, int N>
+__device__ __forceinline__ void stream_vec(T* p, const float (&x)[N]) {
+  __builtin_nontemporal_store(round_vec<T, N>(x), reinterpret_cast<typename mem_vec<T, N>::type*>(p));
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void stream_vec(T* p, const float (&x)[N], int n) {
+  if (n >= N) {
+    stream_vec<T, N>(p, x);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) p[i] = (T)x[i];
 }
 
 template <typename T, int N>
