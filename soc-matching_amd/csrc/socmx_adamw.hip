@@ -82,9 +82,18 @@ __global__ __launch_bounds__(64) void adamw_begin_kernel(float* steps, int n, do
   correction[4 * i + 2] = __uint_as_float((uint32_t)t);
 }
 
-// (the hardware's root and reciprocal, each within one step of f32: two of the update's two dozen roundings)
+// The hardware's root and reciprocal, each within one step of f32: two of the update's two dozen roundings.  The root takes numbers below
+// 2^-126 for 0.  It is off by 2^-63 then, times 32 for the first steps of a decay of 0.999: nothing beside an eps of 1e-10; with less, small
+// numbers are moved up by 2^64 and their root down by 2^-32 (for every eps: 405 us instead of 385 for 96 M 8-bit elements).
 __device__ __forceinline__ float adamw_weight(float p, float m, float v, float size, float root, float decay, float eps) {
-  float w = p * decay - size * m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * root + eps);
+  float deviation;
+  if (eps < 1e-10f) {
+    const bool small = v < 0x1p-100f;
+    deviation = __builtin_amdgcn_sqrtf(v * (small ? 0x1p64f : 1.f)) * (small ? 0x1p-32f : 1.f);
+  } else {
+    deviation = __builtin_amdgcn_sqrtf(v);
+  }
+  float w = p * decay - size * m * __builtin_amdgcn_rcpf(deviation * root + eps);
   asm("" : "+v"(w));      // a float32 from here on: a 16-bit weight is its rounding, not a second result of one mixed instruction
   return w;
 }

@@ -261,14 +261,17 @@ __device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&sum)[
 }
 
 // ---- the chunks in front ----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float plain_nan(float v) { return v != v ? __builtin_nanf("") : v; }      // (never a bit pattern that means empty)
+__device__ __forceinline__ uint32_t filled(float v) {              // never the bits that mean empty (one of the patterns of NaN)
+  const uint32_t u = __float_as_uint(v);
+  return u == kNoState ? 0x7FC00000u : u;
+}
 
 __device__ __forceinline__ void leave_word(uint64_t* p, float q, float l) {
-  const uint64_t v = (uint64_t)__float_as_uint(plain_nan(q)) | (uint64_t)__float_as_uint(l) << 32;
+  const uint64_t v = (uint64_t)filled(q) | (uint64_t)__float_as_uint(l) << 32;
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void leave_state(float* p, float s) {
-  __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(plain_nan(s)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(reinterpret_cast<uint32_t*>(p), filled(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // N words each lane with `need` waits for

@@ -96,6 +96,11 @@ Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Device& dev) {
   return at::empty(size, at::TensorOptions().dtype(type).device(dev));
 }
 
+// what a call wrote in place: a graph that has saved it refuses its backward
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor floats(int64_t n, const at::Device& dev) { return n ? empty({n}, at::kFloat, dev) : Tensor(); }
 
 // the device of the tensors made current, and its current stream
@@ -365,6 +370,7 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
     check(abi.socmx_gated_scan_step(element_type(x), element_type(a), (int32_t)B, (int32_t)D, (int32_t)a.size(1), pointer(x), x.stride(0),
                                     pointer(a), a.stride(0), state.data_ptr<float>(), state.stride(0), pointer(h), l.stream),
           "socmx_gated_scan_step");
+    written(state);
   }
   return h;
 }
@@ -395,6 +401,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
   std::vector<socmx_adamw_tensor> rows(count);
   std::unordered_set<const void*> seen;
+  seen.reserve(5 * count);
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = ms[i], &v = vs[i];
     const Tensor s = scales ? (*scales)[i] : Tensor(), w = masters ? (*masters)[i] : Tensor();
@@ -410,12 +417,22 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
       if (t->defined() && (t->device() != dev || !t->is_contiguous()))
         refuse(what, ": tensor ", i, " has a part on ", t->device(), " with strides ", t->strides(), "; dense ones on ", dev, " are needed");
     if (n && !seen.insert(p.data_ptr()).second) refuse(what, ": the same tensor twice in params");
+    for (const Tensor* t : {&m, &v, &s, &w})
+      if (t->defined() && n && !seen.insert(t->data_ptr()).second) refuse(what, ": the state or master of tensor ", i, " is another tensor's too");
     rows[i] = socmx_adamw_tensor{pointer(p), pointer(g), pointer(m), pointer(v), pointer_as<float>(s), pointer_as<float>(w), n};
   }
   const Tensor ws = floats(4 * (int64_t)count, dev);
   const Launch l(dev);
   check(abi.socmx_adamw_step(element_type(params[0]), scales ? 8 : 32, rows.data(), (int32_t)count, steps.data_ptr<float>(),
                              ws.data_ptr<float>(), lr, b1, b2, eps, weight_decay, l.stream), "socmx_adamw_step");
+  written(steps);
+  for (size_t i = 0; i < count; ++i) {
+    written(params[i]);
+    written(ms[i]);
+    written(vs[i]);
+    if (scales) written((*scales)[i]);
+    if (masters) written((*masters)[i]);
+  }
 }
 
 // a dense tensor of its own over a part of a buffer's storage (which lives as long as one of them does)

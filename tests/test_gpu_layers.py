@@ -932,3 +932,99 @@ def test_the_trainer_with_adamw(graph, bits):
         for (name, p), q in zip(sde.named_parameters(), ref.parameters()):
             # six steps of at most 1e-3 each, whose gradients agree to about 1e-4: where a gradient is near nothing the direction is free
             assert float((p - q).abs().max()) <= 6 * 1e-3 * 0.05 + 1e-6 * float(q.abs().max()), name
+
+
+def test_gated_scan_in_chunks_captured():
+    """A sequence of several chunks, forward and backward in one graph, replayed with other inputs: every replay equals the eager call."""
+    cases = [[t.to(DEV) for t in scan_case(1500, 2, 96, 3, seed, BF16, F32, resets=0.002)] for seed in range(4)]
+    lengths = torch.tensor([1500, 1111], dtype=torch.int32, device=DEV)
+
+    def once(x, a, initial, dh, dfinal):
+        ts = [t.detach().requires_grad_() for t in (x, a, initial)]
+        h, final = layers.gated_scan(*ts, lengths=lengths)
+        return [h.detach(), final.detach()] + list(torch.autograd.grad([h, final], ts, [dh, dfinal]))
+    want = [[t.clone() for t in once(*c)] for c in cases]
+    held = [t.clone() for t in cases[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = once(*held)
+    for i in (0, 1, 2, 3, 1, 0):
+        for t, c in zip(held, cases[i]):
+            t.copy_(c)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want[i])), i
+        assert all(torch.equal(p, q) for p, q in zip(once(*cases[3 - i]), want[3 - i])), i
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_rows_further_apart_than_32_bits_count(kind):
+    """Rows 2^31 elements and more apart, as in a slice of a large buffer."""
+    far = 2 ** 31 + 640
+    big = torch.zeros(2 * far + 4096, dtype=kind, device=DEV)
+    x, a, initial, dh, dfinal = scan_case(150, 3, 16, 2, 77, kind, F32)
+    wide = big.as_strided((150, 3, 16), (20, far, 1))
+    wide.copy_(x)
+    scan_check(wide, a.to(DEV), initial, dh.to(DEV), dfinal)
+    rows = big.as_strided((3, 1000), (far, 1))
+    rows.copy_(dh.reshape(-1)[:3000].reshape(3, 1000))
+    w, b = torch.ones(1000, device=DEV), torch.zeros(1000, device=DEV)
+    assert torch.equal(layers.layer_norm(rows, w, b), layers.layer_norm(rows.contiguous(), w, b))
+
+
+def test_adamw_8_bit_beyond_32_bit_offsets():
+    """The last 1000 of 2^32 + 1000 elements get the codes of the first 1000 of a small tensor: thresholds repeat after 2^32 elements."""
+    n, tail = 2 ** 32 + 1000, 1000
+    g = gen(3)
+    grad, start = (0.1 * torch.randn(tail, generator=g)).to(BF16), torch.randn(tail, generator=g).to(BF16)
+    p, q = (torch.zeros(n, dtype=BF16, device=DEV) for _ in range(2))
+    m, v, scales, _ = new_states([n], BF16, 8, False, [p])
+    ps, qs = start.to(DEV), grad.to(DEV)
+    ms, vs, small, _ = new_states([tail], BF16, 8, False, [ps])
+    p[-tail:], q[-tail:] = ps, qs
+    steps = [torch.zeros(1, device=DEV) for _ in range(2)]
+    for _ in range(2):
+        optim.adamw_step([p], [q], m, v, steps[0], scales=scales, **HYPER)
+        optim.adamw_step([ps], [qs], ms, vs, steps[1], scales=small, **HYPER)
+    for wide, narrow in ((p, ps), (m[0], ms[0]), (v[0], vs[0])):
+        assert torch.equal(wide[-tail:], narrow) and not bool(wide[:tail].any()) and not bool(wide[2 ** 31:2 ** 31 + tail].any())
+    assert torch.equal(scales[0][-4:], small[0])
+
+
+def test_what_is_written_in_place_is_seen_by_autograd():
+    w = torch.ones(4, device=DEV, requires_grad=True)
+    state, one = torch.ones(2, 4, device=DEV), torch.ones(2, 4, device=DEV)
+    y = (w * state).sum()
+    layers.gated_scan_step(state, one, one)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    y = (w * w).sum()
+    with torch.no_grad():
+        optim.adamw_step([w], [torch.ones_like(w)], *new_states([4], F32, 32, False, [w])[:2], torch.zeros(1, device=DEV), lr=1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
+def test_adamw_refuses_shared_states():
+    f = lambda t=F32: torch.zeros(10, dtype=t, device=DEV)   # noqa: E731
+    one = f()
+    ok = dict(params=[f(), f()], grads=[one, one], exp_avgs=[f(), f()], exp_avg_sqs=[f(), f()], steps=torch.zeros(2, device=DEV), lr=1e-3)
+    optim.adamw_step(**ok)                                     # (a gradient is only read: it may be shared)
+    for bad in (dict(exp_avgs=[one, one]), dict(exp_avgs=[one, f()], exp_avg_sqs=[f(), one]), dict(exp_avg_sqs=ok["params"])):
+        with pytest.raises(SocmxError, match="another tensor's"):
+            optim.adamw_step(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("size", [1e-18, 1e-20])
+def test_adamw_of_tiny_gradients_without_eps(size):
+    """The first update is lr whatever the gradient's size.  v = 5e-42 at 1e-20 is 3600 of float32's smallest numbers: g g, its product and
+    the sum are off by half of one each, 2e-4 of v, half of that of its root."""
+    p, g = torch.zeros(300, device=DEV), torch.full((300,), size, device=DEV)
+    m, v, _, _ = new_states([300], F32, 32, False, [p])
+    optim.adamw_step([p], [g], m, v, torch.zeros(1, device=DEV), lr=1e-2, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0)
+    close(p, torch.full((300,), -1e-2).double(), 1e-2 * (30 * U + (2.1e-4 if size < 1e-19 else 0)))
