@@ -14,8 +14,9 @@
 // 16384 elements are read again from the caches instead of being kept (the *_long kernels).
 //
 // MEASURED.  bf16 (8192, 4096): forward 26.5 us (5.1 TB/s), backward 40 (5.0) and 4 for the slots, a copy of this size runs at 5.3 to 6.8;
-// f32 (25728, 256): 12 (4.4), 16 (4.8) and 3.  f16 (4111, 1601), rows at odd addresses: 12, 16 and 5, a third of that rate: one row a workgroup,
+// f32 (25728, 256): 11 (4.8), 16 (4.9) and 3.  f16 (4111, 1601), rows at odd addresses: 12, 16 and 5, a third of that rate: one row a workgroup,
 // all of them at once, so what is left is the way of one row through three sums.  y leaves past the caches (28.5 -> 26.5 us); dx did not gain.
+// The first shape's forward with 8 elements a lane (twice the waves a row) 30 us, with 32 28, alone 24.6; (4111, 1601) 11.0, 13.6 and 10.8.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

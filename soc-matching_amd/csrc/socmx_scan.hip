@@ -33,6 +33,7 @@
 // 20 + 28 otherwise).
 // Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57.  U = 16, W = 8 and
 // kGroup = 16 were the best or within 2 % of it among U 4, 8, 16, W 4, 8, 16 and groups of 16, 32; chunks wait for each other 3 to 7 % of the time.
+// Workgroups that stay and draw their next ticket early hold up whoever waits for it: 283 -> 315 us for the first shape.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -221,16 +222,20 @@ __device__ __forceinline__ void gate_hand(float (&q)[kScanU][1], float g, std::i
 // q of U steps and the sum of their alphas (-inf once a gate forgets); whether one of this wave's gates does.  origin: alpha at step 0.
 // ROW: the 16 lanes of a row share their gate.  Lane u of a row takes step u -- one load and one gate instead of sixteen -- and hands it to the
 // others.
-template <typename TA, int NA, bool ROW>
-__device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&sum)[NA], const TA* origin, int64_t d, int k0, int len, bool full) {
+// meanwhile(): what is loaded behind them.
+template <typename TA, int NA, bool ROW, typename F>
+__device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&sum)[NA], const TA* origin, int64_t d, int k0, int len, bool full, F&& meanwhile) {
   bool cut = false;
   if constexpr (ROW) {
     static_assert(NA == 1 && kScanU == 16, "a gate for a row of 16 lanes, a step for each of them");
     const int u = threadIdx.x & 15;
     const bool in = full || k0 + u < len;
     float g = kGateKeeps, s = 0.f;
+    TA raw = (TA)0.f;
+    if (in) raw = origin[(int64_t)(k0 + u) * d];
+    meanwhile();
     if (in) {
-      s = (float)origin[(int64_t)(k0 + u) * d];
+      s = (float)raw;
       g = gate_of(s);
       cut = g == 0.f;
     }
@@ -241,6 +246,7 @@ __device__ __forceinline__ bool scan_gates(float (&q)[kScanU][NA], float (&sum)[
   } else {
     reg_vec<TA, NA> raw[kScanU];
     scan_load<TA, NA>(raw, origin, d, k0, len, full);
+    meanwhile();
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       bool zero = false;
@@ -417,8 +423,9 @@ __global__ __launch_bounds__(64 * kScanW, 4) void gated_scan_fwd_kernel(const Sc
   float q[kScanU][NA], sum[NA] = {}, h[V];
   bool cut = false;
   if (!none) {
-    scan_load<T, V>(rx, scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c), dx, k0, l.len, full);
-    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c), da, k0, l.len, full);
+    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, NA == 1 ? l.gate : l.c), da, k0, l.len, full, [&] {
+      scan_load<T, V>(rx, scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c), dx, k0, l.len, full);
+    });
   }
   // the run from zero; the steps themselves afterwards, with the same code
   auto walk = [&](auto CUT, auto FULL, auto&& each) {
@@ -539,8 +546,9 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
 #pragma unroll
   for (int u = 0; u < kScanU; ++u) rd[u] = reg_vec<T, V>{};
   if (!none) {
-    if (a.dh) scan_load<T, V>(rd, scan_origin(static_cast<const T*>(a.dh), a, l, a.dht, a.dhb, l.c), dd, k0, l.len, full);
-    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, gate), da, k0, l.len, full);
+    cut = scan_gates<TA, NA, ROW>(q, sum, scan_origin(static_cast<const TA*>(a.alpha), a, l, a.at, a.ab, gate), da, k0, l.len, full, [&] {
+      if (a.dh) scan_load<T, V>(rd, scan_origin(static_cast<const T*>(a.dh), a, l, a.dht, a.dhb, l.c), dd, k0, l.len, full);
+    });
   }
   const bool plain = full && !cut;
   auto value = [&](const reg_vec<T, V>& r, int u, int i, bool all) { return all || k0 + u < l.len ? r[i] : 0.f; };
