@@ -28,8 +28,8 @@
 // floating-point atomics.
 //
 // MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 116 us (4.4 TB/s of x, alpha, h and states) + 160 us (5.3): memory, a copy of
-// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 80 us (3.6 TB/s) + 126 us (3.4); rows that are on average 3/4
-// full 66 + 100, of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 19 + 23.  Results leave past the caches (121 + 170, 84 + 131,
+// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 80 us (3.6 TB/s) + 126 us (3.4); rows of 0 to 4096 steps,
+// 55 % of them in all, 66 + 100 (3.5, 3.1), of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 19 + 23.  Results leave past the caches (121 + 170, 84 + 131,
 // 20 + 28 otherwise).
 // Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57.  U = 16, W = 8 and
 // kGroup = 16 were the best or within 2 % of it among U 4, 8, 16, W 4, 8, 16 and groups of 16, 32; chunks wait for each other 3 to 7 % of the time.
