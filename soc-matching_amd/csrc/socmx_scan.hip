@@ -16,8 +16,8 @@
 // those in front of it from there, and its waves walk their steps from the state they find.  So x and alpha are read once and h is
 // written once, however few channels there are.
 //   Who waits for whom: chunks are dealt out by a ticket in the order of the steps, so a chunk waits only for workgroups that have started
-// and that leave their (q, l) without waiting for anybody.  A chunk takes at most kGroup - 1 of them, in order; the state at every kGroup-th
-// chunk is left by the chunk in front of it, which is the one chain along time.  What is composed with what does not depend on who comes
+// and that leave their (q, l) without waiting for anybody.  A chunk takes a group's chunks at most, in order; the state at every
+// group's first chunk is left by the chunk in front of it, which is the one chain along time.  What is composed with what does not depend on who comes
 // first: the same bits on every run.  A word in memory is its own flag: it is set to kEmpty by a launch before this one, written once by one
 // 64-bit store, and read until it is something else -- no fence, which would write back the cache of a whole die.  A wait that lasts
 // kPolls reads (about a second) ends in NaN: the launch ends whatever happens.
@@ -27,13 +27,12 @@
 // products are summed across the lanes in a fixed order, gates wider than a wave leave one partial sum a wave for another launch.  No
 // floating-point atomics.
 //
-// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 116 us (4.4 TB/s of x, alpha, h and states) + 160 us (5.3): memory, a copy of
-// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 80 us (3.6 TB/s) + 126 us (3.4); rows of 0 to 4096 steps,
-// 55 % of them in all, 66 + 100 (3.5, 3.1), of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 19 + 23.  Results leave past the caches (121 + 170, 84 + 131,
-// 20 + 28 otherwise).
-// Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57.  U = 16, W = 8 and
-// kGroup = 16 were the best or within 2 % of it among U 4, 8, 16, W 4, 8, 16 and groups of 16, 32; chunks wait for each other 3 to 7 % of the time.
-// Workgroups that stay and draw their next ticket early hold up whoever waits for it: 283 -> 315 us for the first shape.
+// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 116 us (4.4 TB/s of x, alpha, h and states) + 163 us (5.2): memory, a copy of
+// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 70 us (4.1 TB/s) + 123 us (3.5); rows of 0 to 4096 steps, 55 % of them in
+// all, 62 + 96 (3.7, 3.2), of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 13 + 23.  Results leave past the caches (5 % less than through them).
+// Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57 us together.  U = 16 was the
+// best among 4, 8, 16; chunks wait for each other 3 to 7 % of the time.  Workgroups that stay and draw their next ticket early hold up
+// whoever waits for it: 283 -> 315 us for the first shape.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -52,7 +51,7 @@ struct ScanArgs {
   const float *initial, *dfinal;     // (B, D), nullable (zeros)
   float *final, *dinitial;           // (B, D), nullable
   float* state;                      // (ceil(T / U), B D): the state in front of every U-th step; written by the forward when not NULL
-  uint64_t* word;                    // (chunks, B D): q and l of every chunk; then (ceil(chunks / kGroup), B D) floats: the state at its first
+  uint64_t* word;                    // (chunks, B D): q and l of every chunk; then (ceil(chunks / group), B D) floats: the state at its first
   float* mark;                       //   chunk; then the ticket (more than one chunk only)
   uint32_t* ticket;
   float* part;                       // (T, B G, segments): partial sums of dalpha (gates wider than a wave only)
@@ -60,7 +59,7 @@ struct ScanArgs {
   int64_t xt, xb, at, ab, ht, hb, dht, dhb;   // elements between steps / rows of x, alpha, h, dh
   int64_t dxt, dxb, dat, dab;                 // of dx, dalpha
   int T, B, D, G, reverse;
-  int chunks;
+  int chunks, group;                 // every group-th chunk has its state marked (group <= kGroup)
   uint32_t blocks;                   // workgroups a chunk
 };
 
@@ -110,7 +109,7 @@ __device__ __forceinline__ float run_apply(float q, float h, float l) {
   return gate_apply<true>(q, gate_keeps(q), h, l);
 }
 
-constexpr int kScanW = 8, kScanU = 16, kScanTile = kScanW * kScanU, kGroup = 16;
+constexpr int kScanU = 16, kGroup = 16;
 constexpr int kPolls = 1 << 20;
 constexpr uint64_t kEmpty = ~0ull;
 constexpr uint32_t kNoState = ~0u;
@@ -316,17 +315,17 @@ __global__ __launch_bounds__(256) void gated_scan_clear_kernel(uint64_t* word, i
   if (i == 0) *ticket = 0;
 }
 
-template <int V, int NA>
+template <int W, int V, int NA>
 struct ScanMeet {                                  // where the waves of a workgroup meet
-  float q[kScanW][NA][64], sum[kScanW][NA][64], l[kScanW][V][64];       // the waves' runs
+  float q[W][NA][64], sum[W][NA][64], l[W][V][64];       // the waves' runs
   float pq[kGroup - 1][V][64], pl[kGroup - 1][V][64];   // the chunks in front, back to the last marked one
   float in[V][64];                                 // the state in front of (behind) the chunk
   uint32_t ticket;
 };
 
 // the number of this workgroup among all of its launch, in the order in which they start
-template <int V, int NA>
-__device__ __forceinline__ uint32_t scan_ticket(const ScanArgs& a, ScanMeet<V, NA>& m) {
+template <int W, int V, int NA>
+__device__ __forceinline__ uint32_t scan_ticket(const ScanArgs& a, ScanMeet<W, V, NA>& m) {
   if (a.chunks == 1) return blockIdx.x;
   if (threadIdx.x == 0) m.ticket = atomicAdd(a.ticket, 1u);
   __syncthreads();
@@ -336,8 +335,8 @@ __device__ __forceinline__ uint32_t scan_ticket(const ScanArgs& a, ScanMeet<V, N
 // The waves' runs (sum, run: this wave's) into the meeting place, and the chunk's (q, l) into memory, for the chunks behind chunk `chunk`
 // (counted in the walk's direction).  The first V waves do that, for one of a lane's channels each.  BACK: the waves' order within the chunk
 // is the opposite one.
-template <int V, int NA, bool BACK>
-__device__ __forceinline__ void scan_leave(ScanMeet<V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, const float (&sum)[NA],
+template <bool BACK, int W, int V, int NA>
+__device__ __forceinline__ void scan_leave(ScanMeet<W, V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, const float (&sum)[NA],
                                            const float (&run)[V], float& chunk_q, float& chunk_l) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -352,25 +351,25 @@ __device__ __forceinline__ void scan_leave(ScanMeet<V, NA>& m, const ScanArgs& a
   if (wave < V) {
     const int gate = NA == 1 ? 0 : wave;
 #pragma unroll
-    for (int k = 0; k < kScanW; ++k) {
-      const int w = BACK ? kScanW - 1 - k : k;
+    for (int k = 0; k < W; ++k) {
+      const int w = BACK ? W - 1 - k : k;
       chunk_q = run_join(chunk_q, m.sum[w][gate][lane]);
       chunk_l = run_apply(m.q[w][gate][lane], chunk_l, m.l[w][wave][lane]);
     }
     chunk_q = run_gate(chunk_q);
-    if (chunk + 1 < a.chunks && (chunk + 1) % kGroup != 0 && l.live)
+    if (chunk + 1 < a.chunks && (chunk + 1) % a.group != 0 && l.live)
       leave_word(a.word + chunk * ((int64_t)a.B * a.D) + l.ch + wave, chunk_q, chunk_l);
   }
 }
 
 // the state in front of the chunk into m.in; first: the state in front of all steps
-template <int V, int NA>
-__device__ __forceinline__ void scan_take(ScanMeet<V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, float chunk_q, float chunk_l,
+template <int W, int V, int NA>
+__device__ __forceinline__ void scan_take(ScanMeet<W, V, NA>& m, const ScanArgs& a, const ScanLane& l, int chunk, float chunk_q, float chunk_l,
                                           const float* first) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t C = (int64_t)a.B * a.D;
-  const int marked = chunk / kGroup * kGroup;
-  for (int j = wave; j < chunk - marked; j += kScanW) {
+  const int marked = chunk / a.group * a.group;
+  for (int j = wave; j < chunk - marked; j += W) {
     float q[V], t[V];
     take_words<V>(q, t, a.word + (marked + j) * C + l.ch, l.live);
 #pragma unroll
@@ -381,7 +380,7 @@ __device__ __forceinline__ void scan_take(ScanMeet<V, NA>& m, const ScanArgs& a,
   }
   float s = 0.f;
   if (wave < V) {
-    if (marked > 0) s = take_state(a.mark + marked / kGroup * C + l.ch + wave, l.live);
+    if (marked > 0) s = take_state(a.mark + marked / a.group * C + l.ch + wave, l.live);
     else if (first && l.live) s = first[l.ch + wave];
   }
   __syncthreads();
@@ -389,35 +388,34 @@ __device__ __forceinline__ void scan_take(ScanMeet<V, NA>& m, const ScanArgs& a,
 #pragma unroll 4
     for (int j = 0; j < chunk - marked; ++j) s = run_apply(m.pq[j][wave][lane], s, m.pl[j][wave][lane]);
     m.in[wave][lane] = s;
-    if (chunk + 1 < a.chunks && (chunk + 1) % kGroup == 0 && l.live)
-      leave_state(a.mark + (chunk + 1) / kGroup * C + l.ch + wave, run_apply(chunk_q, s, chunk_l));
+    if (chunk + 1 < a.chunks && (chunk + 1) % a.group == 0 && l.live)
+      leave_state(a.mark + (chunk + 1) / a.group * C + l.ch + wave, run_apply(chunk_q, s, chunk_l));
   }
   __syncthreads();
 }
 
 // a wave's own state: the chunk's, past the waves in front
-template <int V, int NA, bool BACK>
-__device__ __forceinline__ void scan_own_state(float (&h)[V], const ScanMeet<V, NA>& m) {
+template <bool BACK, int W, int V, int NA>
+__device__ __forceinline__ void scan_own_state(float (&h)[V], const ScanMeet<W, V, NA>& m) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < V; ++i) h[i] = m.in[i][lane];
-  for (int k = 0; k < (BACK ? kScanW - 1 - wave : wave); ++k) {
-    const int w = BACK ? kScanW - 1 - k : k;
+  for (int k = 0; k < (BACK ? W - 1 - wave : wave); ++k) {
+    const int w = BACK ? W - 1 - k : k;
 #pragma unroll
     for (int i = 0; i < V; ++i) h[i] = run_apply(m.q[w][NA == 1 ? 0 : i][lane], h[i], m.l[w][i][lane]);
   }
 }
 
-// (4 waves a SIMD, 97 registers at most: 6 of them at 80 gave 90 us for 84)
-template <typename T, typename TA, int V, int NA, bool ROW>
-__global__ __launch_bounds__(64 * kScanW, 4) void gated_scan_fwd_kernel(const ScanArgs a) {
-  __shared__ ScanMeet<V, NA> meet;
+template <typename T, typename TA, int W, int V, int NA, bool ROW>
+__global__ __launch_bounds__(64 * W, 4) void gated_scan_fwd_kernel(const ScanArgs a) {
+  __shared__ ScanMeet<W, V, NA> meet;
   const uint32_t number = scan_ticket(a, meet);
   const int wave = threadIdx.x >> 6, chunk = number / a.blocks;
   const ScanLane l = scan_lane<V, false>(a, number % a.blocks);
   const int64_t C = (int64_t)a.B * a.D;
   const int64_t dx = a.reverse ? -a.xt : a.xt, da = a.reverse ? -a.at : a.at, dh = a.reverse ? -a.ht : a.ht;
-  const int k0 = (chunk * kScanW + wave) * kScanU;
+  const int k0 = (chunk * W + wave) * kScanU;
   const bool full = __all(k0 + kScanU <= l.len), none = !__any(l.live && k0 < l.len);
   reg_vec<T, V> rx[kScanU];
   float q[kScanU][NA], sum[NA] = {}, h[V];
@@ -445,13 +443,13 @@ __global__ __launch_bounds__(64 * kScanW, 4) void gated_scan_fwd_kernel(const Sc
   if (plain) walk(std::false_type{}, std::true_type{}, [](int) {});
   else if (!none) walk(std::true_type{}, std::false_type{}, [](int) {});
   float chunk_q, chunk_l;
-  scan_leave<V, NA, false>(meet, a, l, chunk, sum, h, chunk_q, chunk_l);
-  scan_take<V, NA>(meet, a, l, chunk, chunk_q, chunk_l, a.initial);
+  scan_leave<false>(meet, a, l, chunk, sum, h, chunk_q, chunk_l);
+  scan_take(meet, a, l, chunk, chunk_q, chunk_l, a.initial);
   scan_forget<NA>(q);
 #pragma unroll
   for (int u = 0; u < kScanU; ++u) scan_forget(rx[u]);
   if (k0 >= a.T) return;
-  scan_own_state<V, NA, false>(h, meet);
+  scan_own_state<false>(h, meet);
   if (a.state && l.live) store_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch, h);
   T* h0 = scan_origin(static_cast<T*>(a.h), a, l, a.ht, a.hb, l.c) + (int64_t)k0 * dh;
   T* pad = static_cast<T*>(a.h) + (int64_t)l.b * a.hb + l.c + (int64_t)k0 * a.ht;        // steps behind the length lie at their own index
@@ -527,9 +525,9 @@ __device__ __forceinline__ float gate_row_sums(const float (&v)[16], int lanes) 
 // GROUPED: a gate has several channels (NA = 1); otherwise every channel has its own (NA = V).  Chunks are counted from the end.
 // 8 bytes a lane and step need 180 to 250 registers, 2 waves a SIMD (3 of them, spilling: 131 -> 163 us); less fits 128 with a
 // step's a_k h_{k-1} kept for half of the steps at a time.
-template <typename T, typename TA, int V, int NA, bool GROUPED, bool ROW>
-__global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated_scan_bwd_kernel(const ScanArgs a) {
-  __shared__ ScanMeet<V, NA> meet;
+template <typename T, typename TA, int W, int V, int NA, bool GROUPED, bool ROW>
+__global__ __launch_bounds__(64 * W, sizeof(T) * V == 8 ? 2 : 4) void gated_scan_bwd_kernel(const ScanArgs a) {
+  __shared__ ScanMeet<W, V, NA> meet;
   const uint32_t number = scan_ticket(a, meet);
   const int wave = threadIdx.x >> 6, chunk = number / a.blocks;
   const ScanLane l = scan_lane<V, GROUPED>(a, number % a.blocks);
@@ -537,7 +535,7 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
   const int64_t dx = a.reverse ? -a.xt : a.xt, da = a.reverse ? -a.at : a.at, dd = a.reverse ? -a.dht : a.dht;
   const int64_t ddx = a.reverse ? -a.dxt : a.dxt, dda = a.reverse ? -a.dat : a.dat;
   const int gate = NA == 1 ? l.gate : l.c;
-  const int k0 = ((a.chunks - 1 - chunk) * kScanW + wave) * kScanU;
+  const int k0 = ((a.chunks - 1 - chunk) * W + wave) * kScanU;
   const bool full = __all(k0 + kScanU <= l.len), none = !__any(l.live && k0 < l.len), begun = k0 < a.T;
   reg_vec<T, V> rx[kScanU], rd[kScanU];
   reg_vec<float, V> rs;
@@ -566,16 +564,16 @@ __global__ __launch_bounds__(64 * kScanW, sizeof(T) * V == 8 ? 2 : 4) void gated
   if (plain) back(std::false_type{}, std::true_type{});
   else if (!none) back(std::true_type{}, std::false_type{});
   float chunk_q, chunk_l;
-  scan_leave<V, NA, true>(meet, a, l, chunk, sum, g, chunk_q, chunk_l);
+  scan_leave<true>(meet, a, l, chunk, sum, g, chunk_q, chunk_l);
   // (x and the state are needed from here on: their way from memory is the wait for the other chunks)
   if (!none) scan_load<T, V>(rx, scan_origin(static_cast<const T*>(a.x), a, l, a.xt, a.xb, l.c), dx, k0, l.len, full);
   if (begun) rs = load_vec<float, V>(a.state + (int64_t)(k0 / kScanU) * C + l.ch);
-  scan_take<V, NA>(meet, a, l, chunk, chunk_q, chunk_l, a.dfinal);
+  scan_take(meet, a, l, chunk, chunk_q, chunk_l, a.dfinal);
   scan_forget<NA>(q);
 #pragma unroll
   for (int u = 0; u < kScanU; ++u) scan_forget(rd[u]);
   if (!begun) return;
-  scan_own_state<V, NA, true>(g, meet);
+  scan_own_state<true>(g, meet);
   const int segs = GROUPED ? (a.D / a.G / V + 63) / 64 : 1;
   TA* const alpha0 = scan_origin(static_cast<TA*>(a.dalpha), a, l, a.dat, a.dab, gate);
   TA* const alpha_pad = static_cast<TA*>(a.dalpha) + (int64_t)l.b * a.dab + gate;
@@ -704,32 +702,43 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const T* __restric
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------
 struct ScanPlan {
-  int V, chunks, segs;
-  int64_t fwd_blocks, bwd_blocks, words;      // words: 64-bit words of workspace for the chunks, the ticket's included
+  int W, V, chunks, group, segs;
+  int64_t blocks, words;               // workgroups a chunk; 64-bit words of workspace for the chunks, the ticket's included
 };
 
-// V channels a lane: up to 8 bytes of x and of gates of their own a step, where they divide the channels of a row (of a gate): for bf16
-// (4096, 8, 2048), 32 decays, 216 us forward and backward with 4 or 2 channels and 286 with 1.
-static ScanPlan scan_plan(const socmx_scan& s) {
+// V channels a lane: up to 8 bytes of x and of gates of their own a step, where they divide the channels of a row (of a gate): the forward of
+// bf16 (4096, 8, 2048), 32 decays, takes 70 us with 4 channels, 88 with 2 and 130 with 1.  One in the backward with gates of their own, two of
+// which spill: 104 us for 113 at bf16 (8192, 4, 1024).
+// W waves a workgroup: 16 in the forward, so that fewer chunks wait for each other -- 80 -> 70 us for the shape above, 40 -> 31 for bf16
+// (30000, 1, 100) with one decay -- but 8 for f32 channels with gates of their own, which fill the memory's time as it is ((65536, 1, 640): 116
+// us for 128), and 8 in the backward, whose registers 16 waves do not have (127 us for 232).
+// group: a chunk takes up to group - 1 chunks and one state.  Where few workgroups make a chunk many chunks are under way, and the chain of
+// states is what they wait for: (30000, 1, 100) backward 44 us with 16, 57 with 8; with many workgroups a chunk shorter takes are better: the first
+// shape's backward 123 us with 8, 127 with 16.
+static ScanPlan scan_plan(const socmx_scan& s, bool bwd) {
   ScanPlan p;
   const int64_t C = (int64_t)s.B * s.D;
   const int per = s.D / s.G;
   p.V = 1;
   const int bytes = (s.type == SOCMX_F32 ? 4 : 2) + (per > 1 ? 0 : s.gate_type == SOCMX_F32 ? 4 : 2);
   for (int v = 4; v > 1; v /= 2)
-    if (bytes * v <= 8 && s.D % v == 0 && (per == 1 || per % v == 0)) { p.V = v; break; }
-  p.fwd_blocks = p.bwd_blocks = (C + 64 * p.V - 1) / (64 * p.V);
+    if (bytes * v <= 8 && s.D % v == 0 && (per == 1 ? !bwd : per % v == 0)) { p.V = v; break; }
+  p.W = bwd || (per == 1 && s.type == SOCMX_F32) ? 8 : 16;
+  p.blocks = (C + 64 * p.V - 1) / (64 * p.V);
   p.segs = 1;
-  if (per > 1) {
+  if (bwd && per > 1) {
     const int wide = per / p.V;
     p.segs = wide <= 64 ? 1 : (wide + 63) / 64;
     const int64_t gates = (int64_t)s.B * s.G;
-    p.bwd_blocks = wide <= 64 ? (gates + 64 / wide - 1) / (64 / wide) : gates * p.segs;
+    p.blocks = wide <= 64 ? (gates + 64 / wide - 1) / (64 / wide) : gates * p.segs;
   }
-  p.chunks = (s.T + kScanTile - 1) / kScanTile;
-  p.words = p.chunks > 1 ? p.chunks * C + ((p.chunks + kGroup - 1) / kGroup * C + 1) / 2 + 1 : 0;
+  p.chunks = (s.T + p.W * kScanU - 1) / (p.W * kScanU);
+  p.group = p.blocks >= 16 ? kGroup / 2 : kGroup;
+  p.words = p.chunks > 1 ? p.chunks * C + ((p.chunks + p.group - 1) / p.group * C + 1) / 2 + 1 : 0;
   return p;
 }
+// (a launch counts its threads in 32 bits)
+static bool scan_fits(const ScanPlan& p) { return p.blocks * p.chunks <= UINT32_MAX / (64 * p.W); }
 
 static int scan_check(const socmx_scan* s) {
   if (!s) return SOCMX_E_NULL;
@@ -744,15 +753,13 @@ static ScanArgs scan_args(const socmx_scan& s, const ScanPlan& p) {
   a.lengths = s.lengths;
   a.xt = s.x_stride_t; a.xb = s.x_stride_b; a.at = s.gate_stride_t; a.ab = s.gate_stride_b;
   a.T = s.T; a.B = s.B; a.D = s.D; a.G = s.G; a.reverse = s.reverse != 0;
-  a.chunks = p.chunks;
+  a.chunks = p.chunks; a.group = p.group; a.blocks = (uint32_t)p.blocks;
   return a;
 }
 
 template <typename T, typename TA, int V, bool BWD>
 static int launch_scan(ScanArgs a, const ScanPlan& p, void* workspace, void* stream) {
   const bool own = a.G == a.D, row = !own && a.D / a.G % (16 * V) == 0;      // (whole rows of lanes share a gate)
-  const int64_t blocks = BWD ? p.bwd_blocks : p.fwd_blocks;
-  a.blocks = (uint32_t)blocks;
   if (p.chunks > 1) {
     const int64_t C = (int64_t)a.B * a.D;
     a.word = static_cast<uint64_t*>(workspace);
@@ -761,24 +768,24 @@ static int launch_scan(ScanArgs a, const ScanPlan& p, void* workspace, void* str
     if (const int err = launch(gated_scan_clear_kernel, dim3((unsigned)((p.words - 1 + 255) / 256)), dim3(256), 0, stream, a.word, p.words - 1, a.ticket))
       return err;
   }
-  const dim3 grid((unsigned)(blocks * p.chunks)), block(64 * kScanW);
+  const dim3 grid((unsigned)(p.blocks * p.chunks)), block(64 * p.W);
   int err = SOCMX_E_DIM;               // (the forms that scan_plan never asks for are not compiled)
-  constexpr bool can_own = (sizeof(T) + sizeof(TA)) * V <= 8, can_share = sizeof(T) * V <= 8;
+  constexpr bool can_own = BWD ? V == 1 : (sizeof(T) + sizeof(TA)) * V <= 8, can_share = sizeof(T) * V <= 8;
   if constexpr (!BWD) {
     if constexpr (can_own)
-      if (own) return launch(gated_scan_fwd_kernel<T, TA, V, V, false>, grid, block, 0, stream, a);
+      if (own) return launch(gated_scan_fwd_kernel<T, TA, sizeof(T) == 4 ? 8 : 16, V, V, false>, grid, block, 0, stream, a);
     if constexpr (can_share)
       if (!own)
-        return row ? launch(gated_scan_fwd_kernel<T, TA, V, 1, true>, grid, block, 0, stream, a)
-                   : launch(gated_scan_fwd_kernel<T, TA, V, 1, false>, grid, block, 0, stream, a);
+        return row ? launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, true>, grid, block, 0, stream, a)
+                   : launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, false>, grid, block, 0, stream, a);
     return err;
   } else {
     if constexpr (can_own)
-      if (own) err = launch(gated_scan_bwd_kernel<T, TA, V, V, false, false>, grid, block, 0, stream, a);
+      if (own) err = launch(gated_scan_bwd_kernel<T, TA, 8, V, V, false, false>, grid, block, 0, stream, a);
     if constexpr (can_share)
       if (!own)
-        err = row ? launch(gated_scan_bwd_kernel<T, TA, V, 1, true, true>, grid, block, 0, stream, a)
-                  : launch(gated_scan_bwd_kernel<T, TA, V, 1, true, false>, grid, block, 0, stream, a);
+        err = row ? launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, true>, grid, block, 0, stream, a)
+                  : launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, false>, grid, block, 0, stream, a);
     if (err || p.segs == 1) return err;
     const int64_t sums = (int64_t)a.T * a.B * a.G;
     return launch(gated_scan_bwd_finish_kernel<TA>, dim3((unsigned)((sums + 255) / 256)), dim3(256), 0, stream, a, p.segs);
@@ -808,12 +815,12 @@ extern "C" int socmx_gated_scan_sizes(const socmx_scan* scan, int64_t* state_flo
                                       int64_t* bwd_workspace_floats) {
   if (const int bad = scan_check(scan)) return bad;
   if (!state_floats || !fwd_workspace_floats || !bwd_workspace_floats) return SOCMX_E_NULL;
-  const ScanPlan p = scan_plan(*scan);
-  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  const ScanPlan f = scan_plan(*scan, false), b = scan_plan(*scan, true);
+  if (!scan_fits(f) || !scan_fits(b)) return SOCMX_E_DIM;
   const int64_t C = (int64_t)scan->B * scan->D;
   *state_floats = (scan->T + kScanU - 1) / kScanU * C;
-  *fwd_workspace_floats = 2 * p.words;
-  *bwd_workspace_floats = 2 * p.words + (p.segs > 1 ? (int64_t)scan->T * scan->B * scan->G * p.segs : 0);
+  *fwd_workspace_floats = 2 * f.words;
+  *bwd_workspace_floats = 2 * b.words + (b.segs > 1 ? (int64_t)scan->T * scan->B * scan->G * b.segs : 0);
   return 0;
 }
 
@@ -822,8 +829,8 @@ extern "C" int socmx_gated_scan_fwd(const socmx_scan* scan, const void* x, const
                                     socmx_stream_t stream) {
   if (const int bad = scan_check(scan)) return bad;
   if (!x || !log_decay || !h) return SOCMX_E_NULL;
-  const ScanPlan p = scan_plan(*scan);
-  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  const ScanPlan p = scan_plan(*scan, false);
+  if (!scan_fits(p)) return SOCMX_E_DIM;
   if (p.chunks > 1 && (!workspace || (uintptr_t)workspace % 8)) return SOCMX_E_WORKSPACE;
   ScanArgs a = scan_args(*scan, p);
   a.x = x; a.alpha = log_decay; a.initial = initial; a.h = h; a.ht = h_stride_t; a.hb = h_stride_b;
@@ -837,8 +844,8 @@ extern "C" int socmx_gated_scan_bwd(const socmx_scan* scan, const void* x, const
                                     float* dinitial, float* workspace, socmx_stream_t stream) {
   if (const int bad = scan_check(scan)) return bad;
   if (!x || !log_decay || !states || !dx || !dlog_decay) return SOCMX_E_NULL;
-  const ScanPlan p = scan_plan(*scan);
-  if (p.chunks * std::max(p.fwd_blocks, p.bwd_blocks) > INT32_MAX) return SOCMX_E_DIM;
+  const ScanPlan p = scan_plan(*scan, true);
+  if (!scan_fits(p)) return SOCMX_E_DIM;
   if ((p.chunks > 1 || p.segs > 1) && (!workspace || (uintptr_t)workspace % 8)) return SOCMX_E_WORKSPACE;
   ScanArgs a = scan_args(*scan, p);
   a.x = x; a.alpha = log_decay; a.state = const_cast<float*>(states); a.dh = dh; a.dht = dh_stride_t; a.dhb = dh_stride_b;

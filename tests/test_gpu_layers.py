@@ -294,6 +294,13 @@ def test_gated_scan_long_time_in_chunks(kind, gkind, T, B, D, G, reverse):
     scan_check(x.to(DEV), a.to(DEV), initial, dh.to(DEV), dfinal, lengths=lengths, reverse=reverse)
 
 
+@pytest.mark.parametrize("kind,T,B,D,G", [(F32, 4500, 2, 600, 600), (BF16, 4500, 1, 4096, 16), (F32, 5000, 1, 20, 20), (BF16, 5000, 1, 20, 4)])
+def test_gated_scan_through_several_groups_of_chunks(kind, T, B, D, G):
+    """Enough steps that the state is handed on from group to group of chunks, for few channels and for many."""
+    x, a, initial, dh, dfinal = scan_case(T, B, D, G, T + D + G, kind, F32, resets=0.0005)
+    scan_check(x.to(DEV), a.to(DEV), initial, dh.to(DEV), dfinal, reverse=D == 600)
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("T,D,G", [(1, 3, 3), (70, 16, 4), (150, 9, 1), (130, 8, 8)])
 def test_gated_scan_padded_batches(T, D, G, reverse):
