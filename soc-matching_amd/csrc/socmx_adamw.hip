@@ -17,9 +17,9 @@
 // than the same formula elsewhere.  A positive v never becomes 0: eps alone would divide m.
 // The weight's update uses m and v as they are before they are rounded.  A block with a value that is not finite gets a NaN scale.
 //
-// MEASURED, 96 M elements: f32 weights, 32 bits 547 us (4.9 TB/s, the rate of a copy of this size); bf16 weights with f32 masters, 8 bits 380 to
-// 425 us (3.6 to 4 TB/s: arithmetic, 123 instructions an
-// element, is 300 us of it, and a copy of as many bytes 314); their decoded values 166 us (5.8 TB/s, most of it stores).  Stores past the caches cost 4 %.  18 tensors, 171 k elements: 6 us.
+// MEASURED, 96 M elements: f32 weights, 32 bits 547 us (4.9 TB/s, the rate of a copy of this size); bf16 weights with f32 masters, 8 bits
+// 363 us (4.2 TB/s, a copy of as many bytes 314; arithmetic, 116 instructions an element, issues for 280 of them); their decoded values 166
+// us (5.8 TB/s, most of it stores).  Stores past the caches cost 4 %.  18 tensors, 171 k elements: 6 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -83,12 +83,14 @@ __global__ __launch_bounds__(64) void adamw_begin_kernel(float* steps, int n, do
   correction[4 * i + 2] = __uint_as_float((uint32_t)t);
 }
 
+__device__ __forceinline__ bool adamw_careful(float eps) { return eps < 1e-10f; }
+
 // The hardware's root and reciprocal, each within one step of f32: two of the update's two dozen roundings.  The root takes numbers below
-// 2^-126 for 0.  It is off by 2^-63 then, times 32 for the first steps of a decay of 0.999: nothing beside an eps of 1e-10; with less, small
+// 2^-126 for 0.  It is off by 2^-63 then, times 32 for the first steps of a decay of 0.999: nothing beside an eps of 1e-10; with less (careful), small
 // numbers are moved up by 2^64 and their root down by 2^-32 (for every eps: 405 us instead of 385 for 96 M 8-bit elements).
-__device__ __forceinline__ float adamw_weight(float p, float m, float v, float size, float root, float decay, float eps) {
+__device__ __forceinline__ float adamw_weight(float p, float m, float v, float size, float root, float decay, float eps, bool careful) {
   float deviation;
-  if (eps < 1e-10f) {
+  if (careful) {
     const bool small = v < 0x1p-100f;
     deviation = __builtin_amdgcn_sqrtf(v * (small ? 0x1p64f : 1.f)) * (small ? 0x1p-32f : 1.f);
   } else {
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
     for (int e = 0; e < 4; ++e) {
       m[e] = b1 * m0[e] + c1 * g[e];
       v[e] = b2 * v0[e] + c2 * (g[e] * g[e]);
-      p[e] = adamw_weight(p[e], m[e], v[e], size, root, a.decay, a.eps);
+      p[e] = adamw_weight(p[e], m[e], v[e], size, root, a.decay, a.eps, adamw_careful(a.eps));
     }
     store_vec<float, 4>(static_cast<float*>(t.m) + i, m, have);
     store_vec<float, 4>(static_cast<float*>(t.v) + i, v, have);
@@ -157,8 +159,16 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t x) {
   x = std::max(x, dpp(x, std::integral_constant<int, 0x4E>{}));     // quad_perm [2,3,0,1]
   x = std::max(x, dpp(x, std::integral_constant<int, 0x141>{}));    // mirror of 8 lanes
   x = std::max(x, dpp(x, std::integral_constant<int, 0x140>{}));    // mirror of 16 lanes
-  x = std::max(x, (uint32_t)__shfl_xor((int)x, 16, 64));
-  return std::max(x, (uint32_t)__shfl_xor((int)x, 32, 64));
+  const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);       // the odd rows of 16 lanes, the even ones
+  x = std::max(rows[0], rows[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return std::max(halves[0], halves[1]);
+}
+
+__device__ __forceinline__ double wave_lane(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 // a block's scale: its maximum, or NaN where that is not finite
@@ -169,6 +179,14 @@ __device__ __forceinline__ float adamw_scale(uint32_t bits) { return bits >= 0x7
 // one for each test that holds -- the same code either way, with no case to tell apart.  `half`: k.
 constexpr float kRootLow = 1.f - 4.8e-7f;                           // (four steps of f32; root and conversion are within two)
 
+// The square of a value that fits 16 bits.  (One full-rate instruction.  The compiler takes the quarter-rate one of 32 bits instead wherever
+// it sees that only low bits are used.)
+__device__ __forceinline__ uint32_t square_small(uint32_t a) {
+  uint32_t r;
+  asm("v_mul_u32_u24_e32 %0, %1, %1" : "=v"(r) : "v"(a));
+  return r;
+}
+
 // (a product of values that fit 24 bits is one full-rate instruction, which looks at no other bits)
 __device__ __forceinline__ uint32_t mul_small(uint32_t a, uint32_t b) {
   return (a & 0xFFFFFFu) * (b & 0xFFFFFFu);
@@ -178,19 +196,19 @@ __device__ __forceinline__ uint32_t mul_small(uint32_t a, uint32_t b) {
 __device__ __forceinline__ int adamw_code_m(double y_scaled, uint32_t half) {
   const uint32_t y = (uint32_t)__builtin_ceil(y_scaled);            // at most 2^17 127^2 and a bit: below 2^31
   const uint32_t c = (uint32_t)(__builtin_amdgcn_sqrtf((float)y) * (0.00276213586400995125f * kRootLow));      // 2^-8.5
-  const uint32_t rest = y - (mul_small(c, c) << 17), gap = 2 * c + 1, odd = 2 * half + 1, first = mul_small(odd, gap);
+  const uint32_t rest = y - (square_small(c) << 17), gap = 2 * c + 1, odd = 2 * half + 1, first = mul_small(odd, gap);
   const uint32_t second = (gap << 17) + first + 2 * odd;            // the gap, and u of the next one, which is 2 wider
   return std::min((int)(c + (rest > first) + (rest > second)), 127);
 }
 
-// y = v / S 255^4: differences of fourth powers need 64 bits, which hold every term exactly
-__device__ __forceinline__ int adamw_code_v(double y, uint32_t half) {
+// y = v / S 255^4: differences of fourth powers need 64 bits, which hold every term exactly.  Everything times 2^17, as above
+__device__ __forceinline__ int adamw_code_v(double y_scaled, uint32_t half) {
 #pragma clang fp contract(off)
-  const uint32_t c = (uint32_t)(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) * kRootLow);           // at most 254
-  const uint32_t c2 = mul_small(c, c), d2 = c2 + 2 * c + 1, e2 = d2 + 2 * c + 3;
+  const uint32_t c = (uint32_t)(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y_scaled)) * (0.0525560259536012f * kRootLow));      // 2^-4.25; at most 254
+  const uint32_t c2 = square_small(c), d2 = c2 + 2 * c + 1, e2 = d2 + 2 * c + 3;
   const uint32_t c4 = mul_small(c2, c2), d4 = mul_small(d2, d2), e4 = mul_small(e2, e2);    // (256^4 wraps to 0, its difference does not)
-  const double u = (double)(2 * half + 1) * (1.0 / 131072.0), rest = y - (double)c4, gap = (double)(d4 - c4);
-  return std::min((int)(c + (rest > u * gap) + (rest > gap + u * (double)(e4 - d4))), 255);
+  const double odd = (double)(2 * half + 1), rest = __builtin_fma(-131072.0, (double)c4, y_scaled), gap = (double)(d4 - c4);
+  return std::min((int)(c + (rest > odd * gap) + (rest > __builtin_fma(odd, (double)(e4 - d4), gap * 131072.0))), 255);
 }
 
 template <typename T>
@@ -203,13 +221,13 @@ struct Adamw8Block {                 // what a lane needs of its four elements
 typedef uint32_t packed_codes __attribute__((aligned(1)));
 
 // `have` of the four elements from `i` on (4 and nothing else where FULL)
-template <typename T, bool FULL>
+template <typename T, bool MASTER, bool FULL>
 __device__ __forceinline__ Adamw8Block<T> adamw8_load(const AdamwTensor& t, int64_t block, int64_t i, int have) {
   Adamw8Block<T> b;
   if (FULL) have = 4;
   const int64_t at = FULL || have ? i : 0;
   b.g = load_vec<T, 4>(static_cast<const T*>(t.g) + at, have);
-  if (t.master) b.p32 = load_vec<float, 4>(t.master + at, have);
+  if constexpr (MASTER) b.p32 = load_vec<float, 4>(t.master + at, have);
   else b.p16 = load_vec<T, 4>(static_cast<T*>(t.p) + at, have);
   const unsigned char *pm = static_cast<unsigned char*>(t.m) + at, *pv = static_cast<unsigned char*>(t.v) + at;
   if (have == 4) {
@@ -226,9 +244,9 @@ __device__ __forceinline__ Adamw8Block<T> adamw8_load(const AdamwTensor& t, int6
   return b;
 }
 
-struct Adamw8Step { double b1, c1, b2, c2; float size, root, decay, eps; uint32_t step; };
+struct Adamw8Step { double b1, c1, b2, c2; float size, root, decay, eps; uint32_t step; bool careful; };
 
-template <typename T, bool FULL>
+template <typename T, bool MASTER, bool FULL>
 __device__ __forceinline__ void adamw8_block(const AdamwTensor& t, const Adamw8Step& h, const Adamw8Block<T>& now, int64_t block, int64_t i, int have) {
 #pragma clang fp contract(off)
   if (FULL) have = 4;
@@ -245,10 +263,13 @@ __device__ __forceinline__ void adamw8_block(const AdamwTensor& t, const Adamw8S
     v[e] = h.b2 * ((double)mul_small(w, w) * kv) + h.c2 * (ge * ge);
     top_m = std::max(top_m, __float_as_uint((float)m[e]) & 0x7FFFFFFFu);
     top_v = std::max(top_v, __float_as_uint((float)v[e]));
-    p[e] = adamw_weight(t.master ? now.p32[e] : now.p16[e], (float)m[e], (float)v[e], h.size, h.root, h.decay, h.eps);
+    p[e] = adamw_weight(MASTER ? now.p32[e] : now.p16[e], (float)m[e], (float)v[e], h.size, h.root, h.decay, h.eps, h.careful);
   }
   const float sm = adamw_scale(wave_max_bits(top_m)), sv = adamw_scale(wave_max_bits(top_v));
-  const double rm = sm > 0.f ? kTopM * (1.0 / (double)sm) * 131072.0 : 0.0, rv = sv > 0.f ? kTopV * (1.0 / (double)sv) : 0.0;
+  // both reciprocals by one division: one half of the wave forms each
+  const float top = threadIdx.x & 32 ? sv : sm;
+  const double inverse = top > 0.f ? 1.0 / (double)top : 0.0;
+  const double rm = kTopM * wave_lane(inverse, 0) * 131072.0, rv = kTopV * wave_lane(inverse, 32) * 131072.0;
   uint32_t cm = 0, cv = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -268,7 +289,7 @@ __device__ __forceinline__ void adamw8_block(const AdamwTensor& t, const Adamw8S
         if (e < have) { pm[e] = (unsigned char)(cm >> (8 * e)); pv[e] = (unsigned char)(cv >> (8 * e)); }
     }
     store_vec<T, 4>(static_cast<T*>(t.p) + i, p, have);
-    if (t.master) store_vec<float, 4>(t.master + i, p, have);
+    if constexpr (MASTER) store_vec<float, 4>(t.master + i, p, have);
   }
   if ((threadIdx.x & 63) == 0) {
     t.scale[2 * block] = sm;
@@ -276,32 +297,40 @@ __device__ __forceinline__ void adamw8_block(const AdamwTensor& t, const Adamw8S
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void adamw8_kernel(const AdamwArgs a) {
-  const int k = adamw_tensor(a.first, a.count, blockIdx.x);
-  const AdamwTensor t = a.tensor[k];
-  const Adamw8Step h = {a.b1, 1.0 - a.b1, a.b2, 1.0 - a.b2, a.correction[4 * k], a.correction[4 * k + 1], a.decay, a.eps,
-                        __float_as_uint(a.correction[4 * k + 2])};
+template <typename T, bool MASTER>
+__device__ __forceinline__ void adamw8_chunk(const AdamwArgs& a, const AdamwTensor& t, int k) {
+  Adamw8Step h = {a.b1, 1.0 - a.b1, a.b2, 1.0 - a.b2, a.correction[4 * k], a.correction[4 * k + 1], a.decay, a.eps,
+                  __float_as_uint(a.correction[4 * k + 2]), adamw_careful(a.eps)};
+  asm("" : "+v"(h.eps));      // (in a vector register: an operation takes one scalar)
   // a wave takes a block of 256 elements at a time, four neighbouring ones a lane; the next block's loads are in flight meanwhile
   const int64_t full = t.n / kAdamwBlock, first = (int64_t)(blockIdx.x - a.first[k]) * (kAdamwChunk / kAdamwBlock);
   const int64_t end = std::min<int64_t>(full, first + kAdamwChunk / kAdamwBlock);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t block = first + wave;
   if (block < end) {
-    Adamw8Block<T> next = adamw8_load<T, true>(t, block, block * kAdamwBlock + lane * 4, 4);
+    Adamw8Block<T> next = adamw8_load<T, MASTER, true>(t, block, block * kAdamwBlock + lane * 4, 4);
 #pragma unroll 1
     for (; block < end; block += 4) {
       const Adamw8Block<T> now = next;
-      if (block + 4 < end) next = adamw8_load<T, true>(t, block + 4, (block + 4) * kAdamwBlock + lane * 4, 4);
-      adamw8_block<T, true>(t, h, now, block, block * kAdamwBlock + lane * 4, 4);
+      if (block + 4 < end) next = adamw8_load<T, MASTER, true>(t, block + 4, (block + 4) * kAdamwBlock + lane * 4, 4);
+      adamw8_block<T, MASTER, true>(t, h, now, block, block * kAdamwBlock + lane * 4, 4);
     }
   }
   // the tensor's last block, where it is not a whole one
   if (block == full && block < first + kAdamwChunk / kAdamwBlock && full * kAdamwBlock < t.n) {
     const int64_t i = block * kAdamwBlock + lane * 4;
     const int have = (int)std::max<int64_t>(0, std::min<int64_t>(4, t.n - i));
-    adamw8_block<T, false>(t, h, adamw8_load<T, false>(t, block, i, have), block, i, have);
+    adamw8_block<T, MASTER, false>(t, h, adamw8_load<T, MASTER, false>(t, block, i, have), block, i, have);
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw8_kernel(const AdamwArgs a) {
+  const int k = adamw_tensor(a.first, a.count, blockIdx.x);
+  const AdamwTensor t = a.tensor[k];
+  if constexpr (sizeof(T) == 2)
+    if (t.master) return adamw8_chunk<T, true>(a, t, k);
+  adamw8_chunk<T, false>(a, t, k);
 }
 
 // 8-bit states as the values they stand for: 2 bytes in, 8 out an element

@@ -13,8 +13,8 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <sstream>
-#include <unordered_set>
 
 #include "../../include/socmx.h"
 
@@ -400,8 +400,8 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
     refuse(what, ": steps is a dense (", count, ",) float32 on ", dev, ", got ", shape(steps), " ", steps.scalar_type(), " on ", steps.device());
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
   std::vector<socmx_adamw_tensor> rows(count);
-  std::unordered_set<const void*> seen;
-  seen.reserve(5 * count);
+  std::vector<const void*> written_to;
+  written_to.reserve(5 * count);
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = ms[i], &v = vs[i];
     const Tensor s = scales ? (*scales)[i] : Tensor(), w = masters ? (*masters)[i] : Tensor();
@@ -416,11 +416,14 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
     for (const Tensor* t : {&p, &g, &m, &v, &s, &w})
       if (t->defined() && (t->device() != dev || !t->is_contiguous()))
         refuse(what, ": tensor ", i, " has a part on ", t->device(), " with strides ", t->strides(), "; dense ones on ", dev, " are needed");
-    if (n && !seen.insert(p.data_ptr()).second) refuse(what, ": the same tensor twice in params");
-    for (const Tensor* t : {&m, &v, &s, &w})
-      if (t->defined() && n && !seen.insert(t->data_ptr()).second) refuse(what, ": the state or master of tensor ", i, " is another tensor's too");
+    if (n)
+      for (const Tensor* t : {&p, &m, &v, &s, &w})
+        if (t->defined()) written_to.push_back(t->data_ptr());
     rows[i] = socmx_adamw_tensor{pointer(p), pointer(g), pointer(m), pointer(v), pointer_as<float>(s), pointer_as<float>(w), n};
   }
+  std::sort(written_to.begin(), written_to.end());
+  if (std::adjacent_find(written_to.begin(), written_to.end()) != written_to.end())
+    refuse(what, ": one of the tensors, states or masters is another tensor's too");
   const Tensor ws = floats(4 * (int64_t)count, dev);
   const Launch l(dev);
   check(abi.socmx_adamw_step(element_type(params[0]), scales ? 8 : 32, rows.data(), (int32_t)count, steps.data_ptr<float>(),

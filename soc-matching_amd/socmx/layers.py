@@ -54,7 +54,8 @@ def gated_scan(x, log_decay, initial=None, lengths=None, reverse=False):
     log_decay may be strided or expanded in their first two dimensions.  initial (B, D) float32, or zeros.
     lengths (B,) int32: row b's steps are the first lengths[b] (0 to T; values outside are clipped); the steps behind them are not
     read, their h and gradients are 0 and the final state is the one before them.  reverse: from each row's last step to its
-    first.  The state and all sums are float32 whatever x's type.  Differentiable in x, log_decay and initial."""
+    first.  The state and all sums are float32 whatever x's type; a state that grows (log_decay above 0) beyond float32 is infinite or NaN, also
+    where the growth of up to 256 steps together is beyond it and the state is not zero.  Differentiable in x, log_decay and initial."""
     return _binding().gated_scan(x, log_decay, initial, lengths, reverse)
 
 
