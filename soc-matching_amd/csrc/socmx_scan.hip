@@ -161,8 +161,7 @@ __device__ __forceinline__ ScanLane scan_lane(const ScanArgs& a, uint32_t block)
     l.c = (int)(l.ch % a.D);
     l.gate = l.c / per;
   }
-  l.len = a.lengths ? min(max(a.lengths[l.b], 0), a.T) : a.T;
-  if (!l.live) l.len = a.T;            // (a lane without channels walks along with channel 0 and stores nothing)
+  l.len = a.lengths ? min(max(a.lengths[l.b], 0), a.T) : a.T;      // (a lane without channels walks along with channel 0 and stores nothing)
   return l;
 }
 
