@@ -46,6 +46,8 @@ def make_optimizer(solver, nabla_V_lr=1e-4, M_lr=1e-2, adam_eps=1e-4, algorithm=
         groups = [{"params": solver.parameters()}]
     # one fused multi-tensor kernel per group on the GPU (same update rule; ~20 launches fewer per iteration)
     on_gpu = next(sde.parameters()).is_cuda
+    if state_bits not in (None, 8, 32):
+        raise ValueError(f"make_optimizer: state_bits is 8 or 32, got {state_bits}")
     if weight_decay or state_bits is not None:
         split = []
         for g in groups:

@@ -138,6 +138,9 @@ def test_make_optimizer_takes_adamw_only_when_asked():
     assert lrs == ref
     with pytest.raises(ValueError, match="8 bits"):
         make_optimizer(solver, state_bits=8)
+    for bits in (0, 16):
+        with pytest.raises(ValueError, match="8 or 32"):
+            make_optimizer(solver, state_bits=bits)
 
 
 def test_the_configuration_has_the_adamw_keys_off():
