@@ -613,6 +613,8 @@ int socmx_gated_scan_step(int32_t type, int32_t gate_type, int32_t B, int32_t D,
  *   codes and scales 0 are states of 0.  socmx_adamw_state_values writes what codes stand for, in f32.
  * steps (ntensors,) f32 device: the updates each tensor has had, advanced by the call (so that a captured call counts its replays).
  * workspace: 4 ntensors floats.  No two tensors may overlap; n may be 0 (the step is counted).
+ * socmx_adamw_step_counts: the same with each tensor's count where it lies (steps: HOST array of ntensors device pointers, read during the
+ *   call), so that a tensor's count keeps its address whichever others are updated with it.
  */
 typedef struct socmx_adamw_tensor {
   void* p;
@@ -634,6 +636,9 @@ typedef struct socmx_adamw_state {
 int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps,
                      float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
                      socmx_stream_t stream);
+int socmx_adamw_step_counts(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* const* steps,
+                            float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
+                            socmx_stream_t stream);
 int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t nstates, socmx_stream_t stream);
 
 #ifdef __cplusplus

@@ -31,7 +31,7 @@
 
 namespace socmx {
 
-constexpr int kAdamwTensors = 48, kAdamwChunk = 4096, kAdamwBlock = 256;
+constexpr int kAdamwTensors = 48, kAdamwChunk = 4096, kAdamwBlock = 256, kAdamwCounts = 256;
 
 struct AdamwTensor {
   void* p;
@@ -72,12 +72,23 @@ __device__ __forceinline__ int adamw_tensor(const int32_t* first, int count, int
   return lo;
 }
 
+// the step counts, next to each other in memory, or each where it lies
+struct AdamwSteps {
+  float* at;
+  __device__ __forceinline__ float* operator[](int i) const { return at + i; }
+};
+struct AdamwCounts {
+  float* at[kAdamwCounts];
+  __device__ __forceinline__ float* operator[](int i) const { return at[i]; }
+};
+
 // 1 - b^t in 64 bits, without cancellation
-__global__ __launch_bounds__(64) void adamw_begin_kernel(float* steps, int n, double log_b1, double log_b2, double lr, float* correction) {
+template <typename Steps>
+__global__ __launch_bounds__(64) void adamw_begin_kernel(const Steps steps, int n, double log_b1, double log_b2, double lr, float* correction) {
   const int i = blockIdx.x * 64 + threadIdx.x;
   if (i >= n) return;
-  const float t = steps[i] + 1.f;
-  steps[i] = t;
+  const float t = *steps[i] + 1.f;
+  *steps[i] = t;
   correction[4 * i] = (float)(lr / -expm1((double)t * log_b1));
   correction[4 * i + 1] = (float)(1.0 / sqrt(-expm1((double)t * log_b2)));
   correction[4 * i + 2] = __uint_as_float((uint32_t)t);
@@ -387,23 +398,36 @@ static inline int64_t adamw_chunks(int64_t n) { return (n + kAdamwChunk - 1) / k
 
 using namespace socmx;
 
-extern "C" int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps,
-                                float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
-                                socmx_stream_t stream) {
-  if (!tensors || !steps || !workspace) return SOCMX_E_NULL;
+// the counts next to each other (steps), or each of them by its address (counts)
+static int adamw_update(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps, float* const* counts,
+                        float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay, void* stream) {
+  if (!tensors || (!steps && !counts) || !workspace) return SOCMX_E_NULL;
   if (type < SOCMX_F32 || type > SOCMX_F16 || (bits != 32 && bits != 8)) return SOCMX_E_KIND;
   if (ntensors < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) return SOCMX_E_DIM;
   for (int i = 0; i < ntensors; ++i) {
     const socmx_adamw_tensor& t = tensors[i];
+    if (counts && !counts[i]) return SOCMX_E_NULL;
     if (t.n < 0 || t.n > (1ll << 40)) return SOCMX_E_DIM;
     if (t.n == 0) continue;
     if (!t.p || !t.grad || !t.exp_avg || !t.exp_avg_sq || (bits == 8 && !t.scale)) return SOCMX_E_NULL;
     if (t.master && type == SOCMX_F32) return SOCMX_E_KIND;
   }
   // (b = 0: log = -inf, expm1 = -1, the correction is 1)
-  if (const int err = launch(adamw_begin_kernel, dim3((ntensors + 63) / 64), dim3(64), 0, stream, steps, (int)ntensors, log(beta1),
-                             log(beta2), lr, workspace))
-    return err;
+  const double log_b1 = log(beta1), log_b2 = log(beta2);
+  if (steps) {
+    if (const int err = launch(adamw_begin_kernel<AdamwSteps>, dim3((ntensors + 63) / 64), dim3(64), 0, stream, AdamwSteps{steps}, (int)ntensors,
+                               log_b1, log_b2, lr, workspace))
+      return err;
+  } else {
+    for (int first = 0; first < ntensors; first += kAdamwCounts) {
+      const int n = std::min(kAdamwCounts, ntensors - first);
+      AdamwCounts some = {};
+      std::copy(counts + first, counts + first + n, some.at);
+      if (const int err = launch(adamw_begin_kernel<AdamwCounts>, dim3((n + 63) / 64), dim3(64), 0, stream, some, n, log_b1, log_b2, lr,
+                                 workspace + 4 * (int64_t)first))
+        return err;
+    }
+  }
   int at = 0;
   while (at < ntensors) {
     AdamwArgs a;
@@ -436,6 +460,18 @@ extern "C" int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_te
     at += count;
   }
   return 0;
+}
+
+extern "C" int socmx_adamw_step(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* steps,
+                                float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                socmx_stream_t stream) {
+  return adamw_update(type, bits, tensors, ntensors, steps, nullptr, workspace, lr, beta1, beta2, eps, weight_decay, stream);
+}
+
+extern "C" int socmx_adamw_step_counts(int32_t type, int32_t bits, const socmx_adamw_tensor* tensors, int32_t ntensors, float* const* steps,
+                                       float* workspace, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                       socmx_stream_t stream) {
+  return adamw_update(type, bits, tensors, ntensors, nullptr, steps, workspace, lr, beta1, beta2, eps, weight_decay, stream);
 }
 
 extern "C" int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t nstates, socmx_stream_t stream) {

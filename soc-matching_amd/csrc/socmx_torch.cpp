@@ -28,7 +28,8 @@ typedef c10::optional<Tensor> Maybe;
 // ---- the C ABI, found in the library that socmx/_lib.py has loaded -----------------------------------------------------------
 #define SOCMX_ABI(X)                                                                                                               \
   X(socmx_layer_norm_fwd) X(socmx_layer_norm_bwd_workspace_floats) X(socmx_layer_norm_bwd) X(socmx_gated_scan_sizes)                 \
-  X(socmx_gated_scan_fwd) X(socmx_gated_scan_bwd) X(socmx_gated_scan_step) X(socmx_adamw_step) X(socmx_adamw_state_values)
+  X(socmx_gated_scan_fwd) X(socmx_gated_scan_bwd) X(socmx_gated_scan_step) X(socmx_adamw_step) X(socmx_adamw_step_counts) \
+  X(socmx_adamw_state_values)
 #define SOCMX_DECLARE(F) decltype(&::F) F;
 struct Abi { SOCMX_ABI(SOCMX_DECLARE) } abi;
 PyObject* socmx_error = nullptr;             // socmx._lib.SocmxError
@@ -379,14 +380,16 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
 typedef std::vector<Tensor> Tensors;
 constexpr int64_t kBlock = 256;
 
-void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& vs, const Tensor& steps, double lr, double b1,
-                double b2, double eps, double weight_decay, const c10::optional<Tensors>& scales, const c10::optional<Tensors>& masters) {
+// steps: one tensor with a count for each of the params, or `counts`: a tensor of one element for each
+void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& vs, const Tensor& steps, const Tensors* counts, double lr,
+                  double b1, double b2, double eps, double weight_decay, const c10::optional<Tensors>& scales, const c10::optional<Tensors>& masters) {
   const char* what = "adamw_step";
   const size_t count = params.size();
   auto same = [&](const char* name, size_t n) { if (n != count) refuse(what, ": ", count, " params and ", n, " ", name); };
   same("grads", grads.size());
   same("exp_avgs", ms.size());
   same("exp_avg_sqs", vs.size());
+  if (counts) same("steps", counts->size());
   if (scales) same("scales", scales->size());
   if (masters) same("masters", masters->size());
   if (count == 0) return;
@@ -396,12 +399,21 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
   if (element_type(params[0]) < 0) refuse(what, ": float32, bfloat16 or float16 weights are needed, got ", type);
   if (masters && type == at::kFloat) refuse(what, ": float32 weights have no masters");
   if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0)) refuse(what, ": betas (", b1, ", ", b2, ") outside [0, 1)");
-  if (steps.dim() != 1 || steps.size(0) != (int64_t)count || steps.scalar_type() != at::kFloat || steps.device() != dev || !steps.is_contiguous())
+  if (!counts && (steps.dim() != 1 || steps.size(0) != (int64_t)count || steps.scalar_type() != at::kFloat || steps.device() != dev || !steps.is_contiguous()))
     refuse(what, ": steps is a dense (", count, ",) float32 on ", dev, ", got ", shape(steps), " ", steps.scalar_type(), " on ", steps.device());
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
   std::vector<socmx_adamw_tensor> rows(count);
   std::vector<const void*> written_to;
-  written_to.reserve(5 * count);
+  written_to.reserve(6 * count);
+  std::vector<float*> at;
+  if (counts)
+    for (size_t i = 0; i < count; ++i) {
+      const Tensor& t = (*counts)[i];
+      if (t.numel() != 1 || t.scalar_type() != at::kFloat || t.device() != dev)
+        refuse(what, ": the step count of tensor ", i, " is one float32 on ", dev, ", got ", shape(t), " ", t.scalar_type(), " on ", t.device());
+      at.push_back(t.data_ptr<float>());
+      written_to.push_back(at.back());
+    }
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = ms[i], &v = vs[i];
     const Tensor s = scales ? (*scales)[i] : Tensor(), w = masters ? (*masters)[i] : Tensor();
@@ -426,16 +438,32 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, 
     refuse(what, ": one of the tensors, states or masters is another tensor's too");
   const Tensor ws = floats(4 * (int64_t)count, dev);
   const Launch l(dev);
-  check(abi.socmx_adamw_step(element_type(params[0]), scales ? 8 : 32, rows.data(), (int32_t)count, steps.data_ptr<float>(),
-                             ws.data_ptr<float>(), lr, b1, b2, eps, weight_decay, l.stream), "socmx_adamw_step");
-  written(steps);
+  const int type_id = element_type(params[0]), bits = scales ? 8 : 32;
+  if (counts)
+    check(abi.socmx_adamw_step_counts(type_id, bits, rows.data(), (int32_t)count, at.data(), ws.data_ptr<float>(), lr, b1, b2, eps, weight_decay,
+                                      l.stream), "socmx_adamw_step_counts");
+  else
+    check(abi.socmx_adamw_step(type_id, bits, rows.data(), (int32_t)count, steps.data_ptr<float>(), ws.data_ptr<float>(), lr, b1, b2, eps,
+                               weight_decay, l.stream), "socmx_adamw_step");
+  if (!counts) written(steps);
   for (size_t i = 0; i < count; ++i) {
+    if (counts) written((*counts)[i]);
     written(params[i]);
     written(ms[i]);
     written(vs[i]);
     if (scales) written((*scales)[i]);
     if (masters) written((*masters)[i]);
   }
+}
+
+void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& vs, const Tensor& steps, double lr, double b1,
+                double b2, double eps, double weight_decay, const c10::optional<Tensors>& scales, const c10::optional<Tensors>& masters) {
+  adamw_update(params, grads, ms, vs, steps, nullptr, lr, b1, b2, eps, weight_decay, scales, masters);
+}
+
+void adamw_step_counts(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& vs, const Tensors& steps, double lr, double b1,
+                       double b2, double eps, double weight_decay, const c10::optional<Tensors>& scales, const c10::optional<Tensors>& masters) {
+  adamw_update(params, grads, ms, vs, Tensor(), &steps, lr, b1, b2, eps, weight_decay, scales, masters);
 }
 
 // a dense tensor of its own over a part of a buffer's storage (which lives as long as one of them does)
@@ -498,5 +526,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_scan", &gated_scan);
   m.def("gated_scan_step", &gated_scan_step);
   m.def("adamw_step", &adamw_step);
+  m.def("adamw_step_counts", &adamw_step_counts);
   m.def("adamw_state_values", &adamw_state_values);
 }

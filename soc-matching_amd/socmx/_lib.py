@@ -152,6 +152,7 @@ PROTOTYPES.update({
     "socmx_gated_scan_step": (C.c_int, [C.c_int32] * 5 + [_fp, C.c_int64, _fp, C.c_int64, _fp, C.c_int64, _fp, _fp]),
     # (the tensors travel as host arrays of 64-bit words: 7 per socmx_adamw_tensor, 6 per socmx_adamw_state)
     "socmx_adamw_step": (C.c_int, [C.c_int32, C.c_int32, _fp, C.c_int32, _fp, _fp] + [C.c_double] * 5 + [_fp]),
+    "socmx_adamw_step_counts": (C.c_int, [C.c_int32, C.c_int32, _fp, C.c_int32, _fp, _fp] + [C.c_double] * 5 + [_fp]),
     "socmx_adamw_state_values": (C.c_int, [_fp, C.c_int32, _fp]),
 })
 

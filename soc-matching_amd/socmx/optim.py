@@ -26,11 +26,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     params, grads: lists of contiguous tensors of ONE type (float32, bfloat16 or float16) on one GPU.  exp_avgs, exp_avg_sqs: float32
     tensors of the same sizes; with `scales`, 8-bit states: int8 and uint8 codes and a float32 (ceil(n / 256), 2) for each tensor of n
     elements (zeros are states of zero; `adamw_state_values` decodes).  masters: float32 weights the update works on, the 16-bit
-    weights getting their rounding.  steps: (len(params),) float32 on the GPU, the updates so far, advanced here -- a captured call
-    counts its replays.  No two tensors may share memory; a tensor may be empty."""
+    weights getting their rounding.  steps: (len(params),) float32 on the GPU, or a list of tensors of one float32 each: the updates so
+    far, advanced here -- a captured call counts its replays.  No two tensors may share memory; a tensor may be empty."""
     if torch.is_tensor(lr):
         raise SocmxError("adamw_step: lr is a number, got a tensor")
-    _lib.torch_binding().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, scales, masters)
+    binding = _lib.torch_binding()
+    call = binding.adamw_step if torch.is_tensor(steps) else binding.adamw_step_counts
+    call(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, scales, masters)
 
 
 def adamw_state_values(exp_avgs, exp_avg_sqs, scales):
@@ -43,8 +45,9 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 32 (float32 states) or 8 (one byte a state, two float32 for 256 elements).  master_weights: keep float32 weights for 16-bit
     parameters (a 16-bit weight does not see updates below 2^-9 of it).  The state is that of torch.optim.AdamW -- "step", "exp_avg",
-    "exp_avg_sq" -- and, where there are any, "scale" and "master".  Parameters without a gradient are left alone.  Step counts live
-    on the GPU, so step() can be captured in a graph once the state exists (one eager step); a learning rate is part of the capture."""
+    "exp_avg_sq" -- and, where there are any, "scale" and "master".  Parameters without a gradient are left alone.  The state of a
+    parameter, its step count included, lives on the GPU and stays where it is, so step() can be captured in a graph once the state exists (one
+    eager step); a learning rate is part of the capture.  load_state_dict makes new state tensors: capture again after it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, master_weights=True):
         if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
@@ -81,20 +84,6 @@ class AdamW(torch.optim.Optimizer):
                 kind = torch.float32 if name == "step" or torch.is_tensor(v) and v.is_floating_point() else None
                 self.state[p][name] = torch.as_tensor(v).detach().clone().to(device=p.device, dtype=kind)
 
-    def _steps(self, found, dev):
-        """The step counts of these parameters as one tensor: their "step" entries are its elements."""
-        base = found[0][1]["step"]._base
-        if base is not None and base.dim() == 1 and base.numel() == len(found) and base.dtype == torch.float32:
-            at = base.data_ptr()
-            if all(st["step"].data_ptr() == at + 4 * i for i, (_, st) in enumerate(found)):
-                return base
-        if torch.cuda.is_current_stream_capturing():
-            raise SocmxError("AdamW: a capture needs a step with the same parameters before it")
-        base = torch.stack([st["step"].reshape(()).to(device=dev, dtype=torch.float32) for _, st in found])
-        for i, (_, st) in enumerate(found):
-            st["step"] = base[i]
-        return base
-
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -110,9 +99,9 @@ class AdamW(torch.optim.Optimizer):
                     raise SocmxError("AdamW: a sparse gradient")
                 st = self.state.get(p) or self._new_state(p, group)
                 kinds.setdefault((p.dtype, p.device, "scale" in st, "master" in st), []).append((p, st))
-            for (_, dev, small, master), found in kinds.items():
+            for (_, _, small, master), found in kinds.items():
                 adamw_step([p for p, _ in found], [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in found],
-                           [st["exp_avg"] for _, st in found], [st["exp_avg_sq"] for _, st in found], self._steps(found, dev),
+                           [st["exp_avg"] for _, st in found], [st["exp_avg_sq"] for _, st in found], [st["step"] for _, st in found],
                            lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                            scales=[st["scale"] for _, st in found] if small else None,
                            masters=[st["master"] for _, st in found] if master else None)

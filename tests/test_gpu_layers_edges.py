@@ -1,0 +1,88 @@
+"""Layer norm, gated scan and AdamW at the edges of what a program does with them: torch's other modes, padded rows whose state is
+infinite, gradients of gradients, rows far from zero, memory that is shared, graphs that outlive a change.
+
+Oracles are plain formulas in 64 bits; tolerances count roundings in units of U = 2^-24, as in test_gpu_layers.py.
+"""
+import math
+
+import pytest
+import torch
+
+from socmx import layers, optim
+from socmx._lib import SocmxError
+from test_gpu_layers import BF16, DEV, F16, F32, HYPER, U, close, gen, half, new_states, scan_case, scan_check, tiny
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_adamw_step_outlives_steps_with_missing_gradients(bits):
+    """Replays of a captured step mixed with eager steps in which a parameter has no gradient: counts, states and weights are those of the
+    same steps made one by one."""
+    sizes, g = (1000, 37, 300), gen(51)
+    start, grads = [torch.randn(n, generator=g) for n in sizes], [[torch.randn(n, generator=g) for n in sizes] for _ in range(12)]
+
+    def setup():
+        ps = [torch.nn.Parameter(t.to(DEV)) for t in start]
+        buffers = [torch.zeros(n, device=DEV) for n in sizes]
+        return ps, buffers, optim.AdamW(ps, lr=1e-2, weight_decay=0.1, state_bits=bits)
+    # (None: all three; k: parameter k has no gradient in this step)
+    plan = [None, None, 1, None, None, 0, 2, None, 1, None, None, None]
+    ps, buffers, opt = setup()
+    cs, held, copt = setup()
+
+    def eager(ps, buffers, opt, row, missing):
+        for i, (p, b, q) in enumerate(zip(ps, buffers, row)):
+            b.copy_(q)
+            p.grad = None if i == missing else b
+        opt.step()
+    graph, side, spare = None, torch.cuda.Stream(), []
+    for k, (row, missing) in enumerate(zip(grads, plan)):
+        eager(ps, buffers, opt, row, missing)
+        if missing is not None or k == 0 or k == 4:
+            eager(cs, held, copt, row, missing)
+        else:
+            for p, b, q in zip(cs, held, row):
+                b.copy_(q)
+                p.grad = b
+            if graph is None:
+                side.wait_stream(torch.cuda.current_stream())
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    copt.step()
+            graph.replay()
+        torch.cuda.synchronize()
+        spare.append(torch.full((128,), 7.0, device=DEV))      # (takes what has been given back to the allocator)
+        for p, c in zip(ps, cs):
+            assert torch.equal(p, c), k
+            for name, v in opt.state[p].items():
+                assert torch.equal(v, copt.state[c][name]), (k, name)
+    assert all(bool((t == 7).all()) for t in spare)
+    assert [float(copt.state[c]["step"]) for c in cs] == [11.0, 10.0, 11.0]
+
+
+def test_adamw_step_counts_each_where_it_lies():
+    """More tensors than one launch counts (256), their counts in any order in one buffer: the same bits as with one tensor of counts."""
+    n, g = 300, gen(52)
+    make = lambda: [torch.randn(3 + i % 5, generator=gen(i)).to(DEV) for i in range(n)]   # noqa: E731
+    grads = [torch.randn(p.shape, generator=g).to(DEV) for p in make()]
+    runs = []
+    for each in (False, True):
+        ps = make()
+        m, v, _, _ = new_states([p.numel() for p in ps], F32, 32, False, ps)
+        steps = torch.arange(n, device=DEV).float()
+        buffer = torch.full((2 * n,), -1.0, device=DEV)
+        buffer[1::2] = steps.flip(0)
+        counts = [buffer[2 * (n - 1 - i) + 1] for i in range(n)]
+        optim.adamw_step(ps, grads, m, v, counts if each else steps, **HYPER)
+        assert torch.equal(torch.stack(counts), torch.arange(n, device=DEV).float() + 1) if each else torch.equal(steps, torch.arange(n, device=DEV).float() + 1)
+        assert bool((buffer[::2] == -1).all())
+        runs.append(ps + m + v)
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    one = torch.zeros((), device=DEV)
+    f = lambda: torch.zeros(10, device=DEV)   # noqa: E731
+    ok = dict(params=[f(), f()], grads=[f(), f()], exp_avgs=[f(), f()], exp_avg_sqs=[f(), f()], lr=1e-3)
+    for bad in ([one, one], [one], [one, f()], [one, torch.zeros(())], [one, one.to(F16)]):
+        with pytest.raises(SocmxError):
+            optim.adamw_step(steps=bad, **ok)
+    assert float(one) == 0.0

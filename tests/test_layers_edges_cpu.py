@@ -1,0 +1,54 @@
+"""Layer operators and AdamW at the edges, without a GPU: torch's other modes, what an optimiser keeps, what the C entry points check."""
+import ctypes as C
+
+import pytest
+import torch
+
+from socmx import _lib, optim
+from socmx._lib import SocmxError
+
+
+def _adamw(rows):
+    flat = [w for row in rows for w in row]
+    return (C.c_int64 * len(flat))(*flat)
+
+
+def test_adamw_keeps_step_counts_where_they_are(monkeypatch):
+    """A captured step holds the addresses of the counts: a step in which a parameter has no gradient must not move them."""
+    calls = []
+
+    class Binding:
+        def adamw_step_counts(self, params, grads, ms, vs, steps, *rest):
+            calls.append([s.data_ptr() for s in steps])
+            for s in steps:
+                s += 1
+    monkeypatch.setattr(_lib, "torch_binding", lambda: Binding())
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (3, 5, 7)]
+    opt = optim.AdamW(params)
+    for p in params:
+        opt.state[p] = dict(step=torch.zeros(()), exp_avg=torch.zeros(p.shape), exp_avg_sq=torch.zeros(p.shape))
+    held = [opt.state[p]["step"] for p in params]
+    for missing in (None, 1, None, 0, None):
+        for i, p in enumerate(params):
+            p.grad = None if i == missing else torch.ones(p.shape)
+        opt.step()
+        assert all(opt.state[p]["step"] is s for p, s in zip(params, held))
+    at = [s.data_ptr() for s in held]
+    assert calls == [at, [at[0], at[2]], at, at[1:], at]
+    assert [float(s) for s in held] == [4.0, 4.0, 5.0]
+
+
+def test_adamw_step_counts_entry_checks():
+    L = _lib.lib()
+    hyper = (1e-3, 0.9, 0.999, 1e-8, 0.01)
+    row = (1, 1, 1, 1, 1, 0, 10)
+    counts = lambda *v: (C.c_int64 * len(v))(*v)   # noqa: E731
+    assert L.socmx_adamw_step_counts(0, 32, _adamw([row]), 1, None, 1, *hyper, None) == -1
+    assert L.socmx_adamw_step_counts(0, 32, _adamw([row, row]), 2, counts(1, 0), 1, *hyper, None) == -1
+    assert L.socmx_adamw_step_counts(0, 16, _adamw([row]), 1, counts(1), 1, *hyper, None) == -3
+    assert L.socmx_adamw_step_counts(0, 32, _adamw([row]), 0, counts(1), 1, *hyper, None) == -2
+    p = torch.zeros(5)
+    with pytest.raises(SocmxError, match="1 params and 2 steps"):
+        optim.adamw_step([p], [p], [p], [p], [p, p], lr=1e-3)
+    with pytest.raises(SocmxError, match="no CPU path"):
+        optim.adamw_step([p], [p], [p], [p], [torch.zeros(())], lr=1e-3)
