@@ -85,6 +85,17 @@ void beside(const char* what, const Tensor& first, const Maybe& t) {
   if (t && t->device() != first.device()) refuse(what, ": tensors on ", first.device(), " and on ", t->device());
 }
 
+// Forward-mode derivatives have no rule here: a dual tensor would lose its tangent without a word.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      refuse(what, ": forward-mode derivatives are not implemented, and an input has a tangent");
+}
+const Tensor* given(const Maybe& t) {
+  static const Tensor none;
+  return t ? &*t : &none;
+}
+
 void floating(const char* what, const Tensor& t) {
   if (element_type(t) < 0) refuse(what, ": float32, bfloat16 or float16 is needed, got ", t.scalar_type());
 }
@@ -189,6 +200,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangent("layer_norm", {&grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const auto wtype = static_cast<at::ScalarType>(ctx->saved_data["wtype"].toInt());
@@ -221,6 +233,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
   const char* what = "layer_norm";
+  no_tangent(what, {&x, given(weight), given(bias)});
   if (x.dim() < 1 || x.size(-1) < 1) refuse(what, ": the last dimension is empty or missing, got shape ", shape(x));
   on_gpu(what, x);
   beside(what, x, weight);
@@ -295,6 +308,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     return {h, final_state};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangent("gated_scan", {&grads[0], &grads[1]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &a = saved[1], &states = saved[2], &lengths = saved[3];
     const at::Device dev = x.device();
@@ -334,6 +348,7 @@ void check_scan(const char* what, const Tensor& x, const Tensor& a, int64_t dims
 
 std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const Maybe& initial, const Maybe& lengths, bool reverse) {
   const char* what = "gated_scan";
+  no_tangent(what, {&x, &a, given(initial)});
   check_scan(what, x, a, 3);
   const int64_t T = x.size(0), B = x.size(1), D = x.size(2);
   beside(what, x, initial);
@@ -356,6 +371,7 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const May
 
 Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) {
   const char* what = "gated_scan_step";
+  no_tangent(what, {&state, &x0, &a0});
   const at::NoGradGuard off;
   check_scan(what, x0, a0, 2);
   beside(what, x0, state);
@@ -402,6 +418,7 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
   if (!counts && (steps.dim() != 1 || steps.size(0) != (int64_t)count || steps.scalar_type() != at::kFloat || steps.device() != dev || !steps.is_contiguous()))
     refuse(what, ": steps is a dense (", count, ",) float32 on ", dev, ", got ", shape(steps), " ", steps.scalar_type(), " on ", steps.device());
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
+  for (size_t i = 0; i < count; ++i) no_tangent(what, {&params[i], &grads[i], &ms[i], &vs[i]});
   std::vector<socmx_adamw_tensor> rows(count);
   std::vector<const void*> written_to;
   written_to.reserve(6 * count);

@@ -11,6 +11,8 @@ uses the graph's own memory) and is bit-reproducible: no atomics.  There is no C
 Gradients inside a captured graph: no autograd graph of the same leaves that was built on another stream may be alive (an output kept
 from an eager iteration).  torch ties a leaf's gradient to the stream of its first graph and would wait for the capture there, which
 ends the process when the capture is closed; a call that is captured in that state raises SocmxError instead.
+
+Derivatives are reverse-mode and first order: an input with a forward-mode tangent raises SocmxError, a second derivative raises RuntimeError.
 """
 import torch
 

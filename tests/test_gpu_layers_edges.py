@@ -86,3 +86,25 @@ def test_adamw_step_counts_each_where_it_lies():
         with pytest.raises(SocmxError):
             optim.adamw_step(steps=bad, **ok)
     assert float(one) == 0.0
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor's tangent is not dropped: the call raises, with and without gradients recorded."""
+    import torch.autograd.forward_ad as fwad
+    x, a, state = torch.randn(4, 2, 6, device=DEV), -torch.rand(4, 2, 3, device=DEV), torch.zeros(2, 6, device=DEV)
+    w = torch.ones(6, device=DEV)
+    for grad in (False, True):
+        with fwad.dual_level(), torch.set_grad_enabled(grad):
+            dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+            for call in (lambda: layers.layer_norm(dual(x)), lambda: layers.layer_norm(x, dual(w), w), lambda: layers.layer_norm(x, w, dual(w)),
+                         lambda: layers.gated_scan(dual(x), a), lambda: layers.gated_scan(x, dual(a)), lambda: layers.gated_scan(x, a, dual(state)),
+                         lambda: layers.gated_scan_step(state, dual(x[0]), a[0]), lambda: layers.gated_scan_step(state, x[0], dual(a[0])),
+                         lambda: layers.gated_scan_step(dual(state), x[0], a[0])):
+                with pytest.raises(SocmxError, match="forward-mode"):
+                    call()
+            layers.layer_norm(x)                               # (a plain tensor while a level is open)
+    x.requires_grad_()
+    for y in (layers.layer_norm(x), layers.gated_scan(x, a)[0], layers.gated_scan(x, a)[1]):
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):          # (from the engine: without its class)
+            torch.autograd.grad(y, x, fwad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    assert not bool(state.any())

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from socmx import _lib, optim
+from socmx import _lib, layers, optim
 from socmx._lib import SocmxError
 
 
@@ -52,3 +52,17 @@ def test_adamw_step_counts_entry_checks():
         optim.adamw_step([p], [p], [p], [p], [p, p], lr=1e-3)
     with pytest.raises(SocmxError, match="no CPU path"):
         optim.adamw_step([p], [p], [p], [p], [torch.zeros(())], lr=1e-3)
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwad
+    x, a = torch.zeros(4, 2, 6), torch.zeros(4, 2, 3)
+    p = torch.zeros(5)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: layers.layer_norm(dual(x)), lambda: layers.layer_norm(x, bias=dual(x[0, 0])), lambda: layers.gated_scan(x, dual(a)),
+                     lambda: layers.gated_scan(x, a, dual(x[0])), lambda: layers.gated_scan_step(x[0], dual(x[0]), a[0])):
+            with pytest.raises(SocmxError, match="forward-mode"):
+                call()
+        with pytest.raises(SocmxError, match="no CPU path"):
+            layers.layer_norm(x)
