@@ -5,12 +5,14 @@
 // took 143 us on the host for 40 us of GPU time, most of it in the engine's worker thread, where Python runs cold.
 // Memory comes from torch's allocator, launches go to the current stream of the tensors' device.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <dlfcn.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -83,6 +85,12 @@ void on_gpu(const char* what, const Tensor& first) {
 
 void beside(const char* what, const Tensor& first, const Maybe& t) {
   if (t && t->device() != first.device()) refuse(what, ": tensors on ", first.device(), " and on ", t->device());
+}
+
+// A trace would record the allocations of a call and none of its launches: what it made would return memory that nobody has written.
+void not_traced(const char* what) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    refuse(what, ": cannot be traced");
 }
 
 // Forward-mode derivatives have no rule here: a dual tensor would lose its tangent without a word.
@@ -233,6 +241,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
   const char* what = "layer_norm";
+  not_traced(what);
   no_tangent(what, {&x, given(weight), given(bias)});
   if (x.dim() < 1 || x.size(-1) < 1) refuse(what, ": the last dimension is empty or missing, got shape ", shape(x));
   on_gpu(what, x);
@@ -348,6 +357,7 @@ void check_scan(const char* what, const Tensor& x, const Tensor& a, int64_t dims
 
 std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const Maybe& initial, const Maybe& lengths, bool reverse) {
   const char* what = "gated_scan";
+  not_traced(what);
   no_tangent(what, {&x, &a, given(initial)});
   check_scan(what, x, a, 3);
   const int64_t T = x.size(0), B = x.size(1), D = x.size(2);
@@ -371,6 +381,7 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const May
 
 Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) {
   const char* what = "gated_scan_step";
+  not_traced(what);
   no_tangent(what, {&state, &x0, &a0});
   const at::NoGradGuard off;
   check_scan(what, x0, a0, 2);
@@ -400,6 +411,7 @@ constexpr int64_t kBlock = 256;
 void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms, const Tensors& vs, const Tensor& steps, const Tensors* counts, double lr,
                   double b1, double b2, double eps, double weight_decay, const c10::optional<Tensors>& scales, const c10::optional<Tensors>& masters) {
   const char* what = "adamw_step";
+  not_traced(what);
   const size_t count = params.size();
   auto same = [&](const char* name, size_t n) { if (n != count) refuse(what, ": ", count, " params and ", n, " ", name); };
   same("grads", grads.size());
@@ -493,6 +505,7 @@ Tensor part_of(const Tensor& flat, int64_t offset, at::IntArrayRef sizes) {
 
 std::pair<Tensors, Tensors> adamw_state_values(const Tensors& ms, const Tensors& vs, const Tensors& scales) {
   const char* what = "adamw_state_values";
+  not_traced(what);
   const size_t count = ms.size();
   if (vs.size() != count || scales.size() != count) refuse(what, ": ", count, ", ", vs.size(), " and ", scales.size(), " tensors");
   std::pair<Tensors, Tensors> out;

@@ -13,6 +13,7 @@ from an eager iteration).  torch ties a leaf's gradient to the stream of its fir
 ends the process when the capture is closed; a call that is captured in that state raises SocmxError instead.
 
 Derivatives are reverse-mode and first order: an input with a forward-mode tangent raises SocmxError, a second derivative raises RuntimeError.
+A call under torch.jit.trace or make_fx raises SocmxError.
 """
 import torch
 

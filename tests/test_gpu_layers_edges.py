@@ -108,3 +108,16 @@ def test_forward_mode_derivatives_are_refused():
         with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):          # (from the engine: without its class)
             torch.autograd.grad(y, x, fwad.make_dual(torch.ones_like(y), torch.ones_like(y)))
     assert not bool(state.any())
+
+
+def test_tracing_is_refused():
+    """torch.jit.trace sees allocations and no kernel: its function would return memory that nobody has written."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, a = torch.randn(4, 2, 6, device=DEV), -torch.rand(4, 2, 3, device=DEV)
+    for f, args in ((lambda x: layers.layer_norm(x), (x,)), (lambda x, a: layers.gated_scan(x, a)[0], (x, a)),
+                    (lambda x, a: layers.gated_scan_step(torch.zeros(2, 6, device=DEV), x[0], a[0]), (x, a))):
+        with pytest.raises(SocmxError, match="trac"):
+            torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(SocmxError, match="trac"):
+            make_fx(f)(*args)
+        f(*args)

@@ -66,3 +66,22 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(SocmxError, match="no CPU path"):
             layers.layer_norm(x)
+
+
+def test_tracing_is_refused():
+    """(In front of every other check: on the CPU too the reason is the trace.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, a, codes = torch.zeros(4, 2, 6), torch.zeros(4, 2, 3), torch.zeros(5, dtype=torch.int8)
+
+    def adamw(x):
+        optim.adamw_step([x], [x], [x], [x], torch.zeros(1), lr=1e-3)
+        return x
+
+    def values(x):
+        return optim.adamw_state_values([codes], [codes.to(torch.uint8)], [torch.zeros(1, 2)])[0][0]
+    for f, args in ((lambda x: layers.layer_norm(x), (x,)), (lambda x, a: layers.gated_scan(x, a)[0], (x, a)),
+                    (lambda x, a: layers.gated_scan_step(x[0].clone(), x[0], a[0]), (x, a)), (adamw, (x,)), (values, (x,))):
+        with pytest.raises(SocmxError, match="cannot be traced"):
+            torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(SocmxError, match="cannot be traced"):
+            make_fx(f)(*args)
