@@ -78,7 +78,8 @@ __device__ __forceinline__ float gate_of(float alpha) {
 }
 __device__ __forceinline__ float gate_keeps(float q) { return q < 0.f ? 1.f : 0.f; }
 
-// the gate of a step that leaves the state as it is (exact for every finite state)
+// the gate of a step that leaves the state as it is: of every finite state (an infinite one times it is not left out of the sum), so the steps
+// behind a row's length are not applied, and runs of nothing but them (run_apply) leave its product away
 static constexpr float kGateKeeps = -1.17549435e-38f;
 
 // a h + x.  CUT: the gate may forget
@@ -106,7 +107,8 @@ __device__ __forceinline__ float run_gate(float sum) {
 }
 __device__ __forceinline__ float run_apply(float q, float h, float l) {
   q = h == 0.f ? 0.f : q;
-  return gate_apply<true>(q, gate_keeps(q), h, l);
+  h = q == 0.f ? 0.f : h;
+  return fmaf(gate_keeps(q), h, fmaf(q, q == kGateKeeps ? 0.f : h, l));
 }
 
 constexpr int kScanU = 16, kGroup = 16;
@@ -430,8 +432,9 @@ __global__ __launch_bounds__(64 * W, 4) void gated_scan_fwd_kernel(const ScanArg
     for (int u = 0; u < kScanU; ++u) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float g = q[u][NA == 1 ? 0 : i], x = decltype(FULL)::value || k0 + u < l.len ? rx[u][i] : 0.f;
-        h[i] = gate_apply<decltype(CUT)::value>(g, gate_keeps(g), h[i], x);
+        const bool in = decltype(FULL)::value || k0 + u < l.len;
+        const float g = q[u][NA == 1 ? 0 : i], next = gate_apply<decltype(CUT)::value>(g, gate_keeps(g), h[i], in ? rx[u][i] : 0.f);
+        h[i] = in ? next : h[i];
       }
       each(u);
     }
@@ -555,7 +558,8 @@ __global__ __launch_bounds__(64 * W, sizeof(T) * V == 8 ? 2 : 4) void gated_scan
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float c = q[u][NA == 1 ? 0 : i], d = value(rd[u], u, i, decltype(FULL)::value);
-        g[i] = gate_times<decltype(CUT)::value>(c, gate_keeps(c), g[i] + d);
+        const float next = gate_times<decltype(CUT)::value>(c, gate_keeps(c), g[i] + d);
+        g[i] = decltype(FULL)::value || k0 + u < l.len ? next : g[i];
       }
   };
 #pragma unroll
@@ -635,7 +639,8 @@ __global__ __launch_bounds__(64 * W, sizeof(T) * V == 8 ? 2 : 4) void gated_scan
         const float c = q[u][NA == 1 ? 0 : i];
         gx[i] = g[i] + value(rd[u], u, i, all);
         galpha[NA == 1 ? 0 : i] += p[u - part * HALF][i] * gx[i];
-        g[i] = gate_times<cuts>(c, gate_keeps(c), gx[i]);
+        const float next = gate_times<cuts>(c, gate_keeps(c), gx[i]);
+        g[i] = all || k < l.len ? next : g[i];
       }
       if (in) {
         stream_vec<T, V>(gx0, gx);

@@ -121,3 +121,31 @@ def test_tracing_is_refused():
         with pytest.raises(SocmxError, match="trac"):
             make_fx(f)(*args)
         f(*args)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("n,T", [(20, 21), (20, 40), (16, 40), (16, 700), (130, 131), (130, 700), (300, 5000)])
+@pytest.mark.parametrize("G", [8, 2, 1])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_gated_scan_padding_keeps_an_infinite_state(kind, n, T, G, reverse):
+    """A state that is infinite after a row's last step, and a gradient that is when it arrives there, are what they are in a batch without
+    padding.  (Decays of 1/e: infinity times them is infinity.)"""
+    D = 8 if G < 8 else G
+    x, _, initial, dh, dfinal = scan_case(n, 2, D, G, n + T, kind)
+    a = torch.full((n, 2, G), -1.0)
+    last = 0 if reverse else n - 1
+    x[last, 0, 0], x[last, 1, D - 1] = math.inf, -math.inf
+    dfinal[0, 1], dfinal[1, 0] = math.inf, -math.inf
+
+    def run(x, a, dh, lengths):
+        ts = [t.to(DEV).requires_grad_() for t in (x, a, initial)]
+        h, final = layers.gated_scan(*ts, lengths=lengths, reverse=reverse)
+        return [h[:n], final] + [t[:n] for t in torch.autograd.grad([h, final], ts, [dh.to(DEV), dfinal.to(DEV)])]
+    wide = lambda t: torch.cat([t, torch.full((T - n,) + t.shape[1:], math.nan, dtype=t.dtype)])   # noqa: E731
+    want = run(x, a, dh, None)
+    got = run(wide(x), wide(a), wide(dh), torch.tensor([n, n], dtype=torch.int32, device=DEV))
+    assert float(want[1][0, 0]) == math.inf and float(want[1][1, D - 1]) == -math.inf and not bool(want[1].isnan().any())
+    for p, q in zip(got, want):
+        assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.isinf(), q.isinf())
+        p, q = p.nan_to_num(posinf=1.0, neginf=-1.0).double(), q.nan_to_num(posinf=1.0, neginf=-1.0).double()
+        assert float((p - q).abs().max()) <= 64 * U * float(q.abs().max())
