@@ -106,9 +106,8 @@ __device__ __forceinline__ float run_gate(float sum) {
   return q == 0.f && sum != -__builtin_inff() ? 1.17549435e-38f : q;
 }
 __device__ __forceinline__ float run_apply(float q, float h, float l) {
-  q = h == 0.f ? 0.f : q;
-  h = q == 0.f ? 0.f : h;
-  return fmaf(gate_keeps(q), h, fmaf(q, q == kGateKeeps ? 0.f : h, l));
+  const float v = fmaf(gate_keeps(q), h, fmaf(q, q == kGateKeeps ? 0.f : h, l));
+  return h == 0.f || q == 0.f ? l : v;             // (what hangs on h is short: runs are joined one after the other)
 }
 
 constexpr int kScanU = 16, kGroup = 16;
