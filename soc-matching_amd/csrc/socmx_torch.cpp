@@ -270,10 +270,12 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
 // ---- gated scan --------------------------------------------------------------------------------------------------------------------
 Tensor dense_last(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
-// a new tensor of `t`'s shape with steps outside rows, or rows outside steps, as in `t`: whichever it has further apart
+// a new tensor of `t`'s shape with steps outside rows, or rows outside steps, as in `t`: whichever it has further apart.  (No view of another
+// tensor: what a node returns as a view may not be changed in place.)
 Tensor laid_like(const Tensor& t) {
-  if (t.stride(0) < t.stride(1)) return empty({t.size(1), t.size(0), t.size(2)}, t.scalar_type(), t.device()).transpose(0, 1);
-  return empty(t.sizes(), t.scalar_type(), t.device());
+  const int64_t T = t.size(0), B = t.size(1), D = t.size(2);
+  const bool rows_outside = t.stride(0) < t.stride(1);
+  return at::empty_strided({T, B, D}, {rows_outside ? D : B * D, rows_outside ? T * D : D, 1}, t.options().requires_grad(false));
 }
 
 socmx_scan descriptor(const Tensor& x, const Tensor& a, const Tensor& lengths, bool reverse) {

@@ -149,3 +149,25 @@ def test_gated_scan_padding_keeps_an_infinite_state(kind, n, T, G, reverse):
         assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.isinf(), q.isinf())
         p, q = p.nan_to_num(posinf=1.0, neginf=-1.0).double(), q.nan_to_num(posinf=1.0, neginf=-1.0).double()
         assert float((p - q).abs().max()) <= 64 * U * float(q.abs().max())
+
+
+@pytest.mark.parametrize("order", ["time", "batch"])
+def test_gated_scan_results_may_be_changed_in_place(order):
+    """Whatever the layout of x: h and the final state are tensors of their own."""
+    x, a, initial, dh, _ = (t.to(DEV) for t in scan_case(30, 3, 8, 2, 5))
+    if order == "batch":
+        x = x.transpose(0, 1).contiguous().transpose(0, 1)
+    x.requires_grad_()
+    extra = torch.ones(8, device=DEV, requires_grad=True)
+    want, = torch.autograd.grad(layers.gated_scan(x, a, initial)[0], x, 2 * dh)
+    h, final = layers.gated_scan(x, a, initial)
+    assert h._base is None and final._base is None
+    h *= 2
+    final += 1
+    h += extra
+    got, ge = torch.autograd.grad(h, [x, extra], dh)
+    assert torch.equal(got, want)
+    close(ge, dh.double().sum((0, 1)), 90 * U * dh.abs().double().sum((0, 1)))
+    h, _ = layers.gated_scan(x.detach(), a, initial)
+    h += extra                                                 # (no gradients recorded by the scan itself)
+    assert h.requires_grad and h.transpose(0, 1).is_contiguous() is (order == "batch")
