@@ -156,12 +156,16 @@ void refuse_foreign_leaves(const char* what, const at::Device& dev, std::initial
 }
 
 // What a backward returns cannot be differentiated again.  Under create_graph it gets a node that raises and that lies on the way to
-// everything the backward depends on: a second derivative raises, it does not leave terms out.
-variable_list once(const char* what, variable_list out, const variable_list& inputs) {
+// everything the backward depends on -- the gradients it got, and whatever the node that runs has a way to: all of the forward's inputs, also
+// those of which the forward saved a copy or nothing -- so that a second derivative raises and does not leave terms out.
+variable_list once(const char* what, variable_list out, const variable_list& upstream) {
   if (!at::GradMode::is_enabled()) return out;
   torch::autograd::edge_list edges;
-  for (const Tensor& t : inputs)
+  for (const Tensor& t : upstream)
     if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  if (const auto node = torch::autograd::get_current_node())
+    for (const auto& edge : node->next_edges())
+      if (edge.is_valid()) edges.push_back(edge);
   if (edges.empty()) return out;
   const auto node = std::make_shared<torch::autograd::Error>(std::string(what) + ": its backward is not differentiable", std::move(edges));
   for (Tensor& t : out) {
@@ -225,7 +229,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (rows == 0) {
       if (need_w) dw.zero_();
       if (need_b) db.zero_();
-      return once("layer_norm", {dx, dw, db, Tensor()}, {x, w, grads[0]});
+      return once("layer_norm", {dx, dw, db, Tensor()}, grads);
     }
     const int type = element_type(x), wkind = wtype == at::kFloat ? SOCMX_F32 : type;
     if (need_w || need_b) ws = floats(abi.socmx_layer_norm_bwd_workspace_floats(type, rows, cols), dev);
@@ -235,7 +239,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       check(abi.socmx_layer_norm_bwd(type, wkind, pointer(r), rows, cols, r.stride(0), pointer(d), d.stride(0), pointer(w), s, s + rows,
                                      pointer(dx), pointer(dw), pointer(db), pointer_as<float>(ws), l.stream), "socmx_layer_norm_bwd");
     }
-    return once("layer_norm", {dx, dw, db, Tensor()}, {x, w, grads[0]});
+    return once("layer_norm", {dx, dw, db, Tensor()}, grads);
   }
 };
 
@@ -337,7 +341,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                                      pointer(da), da.stride(0), da.stride(1), pointer_as<float>(dinitial), pointer_as<float>(ws), l.stream),
             "socmx_gated_scan_bwd");
     }
-    return once("gated_scan", {dx, da, dinitial, Tensor(), Tensor()}, {x, a, grads[0], grads[1]});
+    return once("gated_scan", {dx, da, dinitial, Tensor(), Tensor()}, grads);
   }
 };
 

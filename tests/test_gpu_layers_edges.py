@@ -171,3 +171,37 @@ def test_gated_scan_results_may_be_changed_in_place(order):
     h, _ = layers.gated_scan(x.detach(), a, initial)
     h += extra                                                 # (no gradients recorded by the scan itself)
     assert h.requires_grad and h.transpose(0, 1).is_contiguous() is (order == "batch")
+
+
+def test_a_second_derivative_is_refused_on_every_way_to_the_inputs():
+    """Also where the upstream gradient is a constant and an input had to be laid out afresh, and by way of the initial state."""
+    g = gen(17)
+    base, decay = torch.randn(2, 8, 5, generator=g).to(DEV).requires_grad_(), (-torch.rand(2, 4, 5, generator=g)).to(DEV).requires_grad_()
+    init = torch.randn(2, 8, generator=g).to(DEV).requires_grad_()
+    far = lambda t: t.permute(2, 0, 1)   # noqa: E731  (steps, rows, channels, the steps next to each other in memory)
+    cases = [(far(base), far(decay), None), (far(base), far(decay).contiguous(), init), (far(base).contiguous(), far(decay), init),
+             (far(base.detach()), far(decay.detach()).requires_grad_(), init), (far(base).contiguous(), far(decay.detach()), init)]
+    for x, a, first in cases:
+        ins = [t for t in (x, a, first) if t is not None and t.requires_grad]
+        h, final = layers.gated_scan(x, a, first)
+        for grad in torch.autograd.grad(h.sum() + final.sum(), ins, create_graph=True):
+            assert grad.requires_grad
+            for t in ins:
+                with pytest.raises(RuntimeError, match="not differentiable"):
+                    torch.autograd.grad(h.sum() + grad.square().sum(), t, retain_graph=True)
+    wide = torch.randn(16, generator=g).to(DEV).requires_grad_()
+    x = torch.randn(3, 8, generator=g).to(DEV)
+    w = wide[::2]
+    y = layers.layer_norm(x, w)
+    grad, = torch.autograd.grad(y.sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum() + grad.square().sum(), wide)
+    x = torch.randn(8, 3, generator=g).to(DEV).requires_grad_()
+    y = layers.layer_norm(x.t(), w)
+    grad, = torch.autograd.grad(y.sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum() + grad.square().sum(), x)
+    # one derivative, by either way, is what it was
+    ref = torch.autograd.grad(layers.gated_scan(far(base), far(decay), init)[0].square().sum(), [base, decay, init])
+    far_dense = torch.autograd.grad(layers.gated_scan(far(base).contiguous(), far(decay).contiguous(), init)[0].square().sum(), [base, decay, init])
+    assert all(torch.equal(p, q) for p, q in zip(ref, far_dense))
