@@ -7,7 +7,8 @@
 // is read ONCE into the registers of the L lanes that own it (at most 16 elements a lane), the variance is the sum of squared
 // differences from the mean (no cancellation of large squares), and the mean of those differences -- what rounding left of the mean,
 // times 1 / sqrt(eps) an error of its own where a row hardly varies -- is taken off once more with the same reduction; all statistics
-// are f32.  L is a power of two: several short
+// are f32.  The mean that is kept for the backward is one f32, which does not hold that rest: there n = (x - mean) r has a mean c of its own,
+// formed beside the other two sums of a row and taken off, n - c (and mean(g n) - c mean(g)).  L is a power of two: several short
 // rows share a wave, rows of more than 1024 elements take L / 64 waves that meet in LDS.  In the backward every lane keeps
 // the weight and bias gradients of its columns over all the rows its workgroup takes; the workgroup's sums go to a slot of
 // their own and a second launch adds the slots in a fixed order: no atomics, the same bits on every run.  Rows of more than
@@ -33,6 +34,7 @@ struct NormArgs {
   void *y, *dx, *dw, *db;            // y of the forward; dx, dw, db of the backward, each nullable
   float *mean, *rstd;                // (rows,); nullable together in the forward
   float* part;                       // backward: (slots, 2, cols)
+  float* shift;                      // backward of long rows: (rows,), the c of every row (with part only)
   int64_t rows, x_stride, dy_stride; // elements between rows; y and dx are dense
   int cols, w32;
   float eps;
@@ -55,26 +57,23 @@ __device__ __forceinline__ void load_weight(float (&out)[VEC], const void* w, in
   }
 }
 
-// totals of two sums over the L lanes (L / 64 waves) of a row; `red`: 2 L / 64 floats, free again after the next call's barrier
-template <int L>
-__device__ __forceinline__ void row_sums(float& s, float& q, float* red) {
-  if constexpr (L <= 64) {
-    s = lanes_sum<L>(s);
-    q = lanes_sum<L>(q);
-  } else {
-    constexpr int W = L / 64;
-    s = lanes_sum<64>(s);
-    q = lanes_sum<64>(q);
+// totals of N sums over the L lanes (L / 64 waves) of a row; `red`: N L / 64 floats, free again after the next call's barrier
+template <int L, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float* red) {
+  constexpr int W = L <= 64 ? 1 : L / 64;
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = lanes_sum<(L <= 64 ? L : 64)>(s[k]);
+  if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) {
-      red[threadIdx.x >> 6] = s;
-      red[W + (threadIdx.x >> 6)] = q;
+#pragma unroll
+      for (int k = 0; k < N; ++k) red[k * W + (threadIdx.x >> 6)] = s[k];
     }
     __syncthreads();
-    s = q = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      s += red[i];
-      q += red[W + i];
+    for (int k = 0; k < N; ++k) {
+      s[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) s[k] += red[k * W + i];
     }
   }
 }
@@ -94,29 +93,28 @@ __global__ __launch_bounds__(L <= 64 ? 256 : L) void layer_norm_fwd_kernel(const
   }
   for (int64_t row = first; row < a.rows; row += stride) {      // (L > 64: the same rows for the whole workgroup)
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    float e[NV][VEC], s = 0.f, q = 0.f, none = 0.f;
+    float e[NV][VEC], s[1] = {}, d[2] = {};              // sums of x; of x - mean and of its square
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int col = (v * L + lane) * VEC;
       reg_vec<T, VEC> raw = load_vec<T, VEC>(x + (col < a.cols ? col : 0), col < a.cols ? a.cols - col : 0);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += e[v][i] = raw[i];
+      for (int i = 0; i < VEC; ++i) s[0] += e[v][i] = raw[i];
     }
-    row_sums<L>(s, none, red[0]);
-    const float mean = s / cols;
-    s = 0.f;
+    row_sums<L>(s, red[0]);
+    const float mean = s[0] / cols;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         e[v][i] -= mean;
         if ((v * L + lane) * VEC + i < a.cols) {
-          s += e[v][i];
-          q += e[v][i] * e[v][i];
+          d[0] += e[v][i];
+          d[1] += e[v][i] * e[v][i];
         }
       }
-    row_sums<L>(s, q, red[1]);
-    const float rest = s / cols, var = q / cols - rest * rest, r = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    row_sums<L>(d, red[1]);
+    const float rest = d[0] / cols, var = d[1] / cols - rest * rest, r = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
     T* y = static_cast<T*>(a.y) + row * a.cols;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -132,11 +130,14 @@ __global__ __launch_bounds__(L <= 64 ? 256 : L) void layer_norm_fwd_kernel(const
   }
 }
 
-// WEIGHTS: the gradients of weight and bias are wanted
+// n here is (x - mean) r, its mean c is known after a row's sums: dx has c in what is the same for the whole row, dw gets its share then.
+// WEIGHTS: the gradients of weight and bias are wanted.  Which operations are fused is written down, so that a gradient has the same bits
+// whichever others are wanted with it.
 template <typename T, int VEC, int NV, int L, bool WEIGHTS>
 __global__ __launch_bounds__(L <= 64 ? 256 : L) void layer_norm_bwd_kernel(const NormArgs a) {
+#pragma clang fp contract(off)
   constexpr int THREADS = L <= 64 ? 256 : L, GROUPS = THREADS / L, WAVES = THREADS / 64;
-  __shared__ float red[2][2 * (L <= 64 ? 1 : L / 64)];
+  __shared__ float red[2][3 * (L <= 64 ? 1 : L / 64)];
   const int lane = threadIdx.x % L;
   const int64_t first = (int64_t)blockIdx.x * GROUPS + threadIdx.x / L, stride = (int64_t)gridDim.x * GROUPS;
   const float inv = 1.f / (float)a.cols;
@@ -152,36 +153,40 @@ __global__ __launch_bounds__(L <= 64 ? 256 : L) void layer_norm_bwd_kernel(const
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     const float mean = a.mean[row], r = a.rstd[row];
-    float n[NV][VEC], g[NV][VEC], s = 0.f, q = 0.f;
+    float n[NV][VEC], sum[3] = {};                       // sums of g, of g n and of n
+    reg_vec<T, VEC> rd[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int col = (v * L + lane) * VEC;
       const int have = col < a.cols ? a.cols - col : 0;
-      const reg_vec<T, VEC> rx = load_vec<T, VEC>(x + (have ? col : 0), have), rd = load_vec<T, VEC>(dy + (have ? col : 0), have);
+      const reg_vec<T, VEC> rx = load_vec<T, VEC>(x + (have ? col : 0), have);
+      rd[v] = load_vec<T, VEC>(dy + (have ? col : 0), have);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {               // (behind the row's end dy = 0: every term below is 0)
+      for (int i = 0; i < VEC; ++i) {               // (behind the row's end dy = 0: what has it for a factor is 0)
         n[v][i] = (rx[i] - mean) * r;
         if constexpr (WEIGHTS) {
-          dw[v][i] += rd[i] * n[v][i];
-          db[v][i] += rd[i];
+          dw[v][i] = fmaf(rd[v][i], n[v][i], dw[v][i]);
+          db[v][i] += rd[v][i];
         }
-        g[v][i] = rd[i] * w[v][i];
-        s += g[v][i];
-        q += g[v][i] * n[v][i];
+        const float g = rd[v][i] * w[v][i];
+        sum[0] += g;
+        sum[1] = fmaf(g, n[v][i], sum[1]);
+        sum[2] += i < have ? n[v][i] : 0.f;
       }
     }
-    if (a.dx) {
-      row_sums<L>(s, q, red[turn]);
-      s *= inv;
-      q *= inv;
-      T* dx = static_cast<T*>(a.dx) + row * a.cols;
+    row_sums<L>(sum, red[turn]);
+    const float s = sum[0] * inv, c = sum[2] * inv, q = fmaf(-c, s, sum[1] * inv), both = fmaf(-c, q, s);
+    T* dx = static_cast<T*>(a.dx) + row * a.cols;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int col = (v * L + lane) * VEC;
+    for (int v = 0; v < NV; ++v) {
+      const int col = (v * L + lane) * VEC;
+      float e[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) g[v][i] = r * (g[v][i] - s - n[v][i] * q);
-        if (col < a.cols) store_vec<T, VEC>(dx + col, g[v], a.cols - col);
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (WEIGHTS) dw[v][i] = fmaf(-c, rd[v][i], dw[v][i]);
+        e[i] = r * fmaf(-n[v][i], q, fmaf(rd[v][i], w[v][i], -both));
       }
+      if (a.dx && col < a.cols) store_vec<T, VEC>(dx + col, e, a.cols - col);
     }
   }
   if constexpr (WEIGHTS) {
@@ -234,26 +239,25 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
   const float cols = (float)a.cols;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    float s = 0.f, q = 0.f, none = 0.f;
+    float s[1] = {}, d[2] = {};
     for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       const reg_vec<T, VEC> v = load_vec<T, VEC>(x + col, a.cols - col);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += v[i];
+      for (int i = 0; i < VEC; ++i) s[0] += v[i];
     }
-    row_sums<1024>(s, none, red[0]);
-    const float mean = s / cols;
-    s = 0.f;
+    row_sums<1024>(s, red[0]);
+    const float mean = s[0] / cols;
     for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       const reg_vec<T, VEC> v = load_vec<T, VEC>(x + col, a.cols - col);
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (col + i < a.cols) {
-          s += v[i] - mean;
-          q += (v[i] - mean) * (v[i] - mean);
+          d[0] += v[i] - mean;
+          d[1] += (v[i] - mean) * (v[i] - mean);
         }
     }
-    row_sums<1024>(s, q, red[1]);
-    const float rest = s / cols, var = q / cols - rest * rest, r = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    row_sums<1024>(d, red[1]);
+    const float rest = d[0] / cols, var = d[1] / cols - rest * rest, r = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
     T* y = static_cast<T*>(a.y) + row * a.cols;
     for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       const reg_vec<T, VEC> v = load_vec<T, VEC>(x + col, a.cols - col);
@@ -273,32 +277,35 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const NormArgs a) {
-  __shared__ float red[2][32];
+  __shared__ float red[2][48];
   const float inv = 1.f / (float)a.cols;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     const float mean = a.mean[row], r = a.rstd[row];
-    float s = 0.f, q = 0.f, w[VEC], e[VEC];
+    float sum[3] = {}, w[VEC], e[VEC];
     for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       const reg_vec<T, VEC> vx = load_vec<T, VEC>(x + col, a.cols - col), vd = load_vec<T, VEC>(dy + col, a.cols - col);
       load_weight<T, VEC>(w, a.w, a.w32, col, a.cols, 1.f);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        s += vd[i] * w[i];
-        q += vd[i] * w[i] * ((vx[i] - mean) * r);
+        const float n = (vx[i] - mean) * r, g = vd[i] * w[i];
+        sum[0] += g;
+        sum[1] += g * n;
+        sum[2] += i < a.cols - col ? n : 0.f;
       }
     }
-    row_sums<1024>(s, q, red[turn]);
-    s *= inv;
-    q *= inv;
+    row_sums<1024>(sum, red[turn]);
+    const float s = sum[0] * inv, c = sum[2] * inv, q = sum[1] * inv - c * s;
+    if (a.shift && threadIdx.x == 0) a.shift[row] = c;
+    if (!a.dx) continue;
     T* dx = static_cast<T*>(a.dx) + row * a.cols;
     for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       const reg_vec<T, VEC> vx = load_vec<T, VEC>(x + col, a.cols - col), vd = load_vec<T, VEC>(dy + col, a.cols - col);
       load_weight<T, VEC>(w, a.w, a.w32, col, a.cols, 1.f);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = r * (vd[i] * w[i] - s - (vx[i] - mean) * r * q);
+      for (int i = 0; i < VEC; ++i) e[i] = r * (vd[i] * w[i] - s - ((vx[i] - mean) * r - c) * q);
       store_vec<T, VEC>(dx + col, e, a.cols - col);
     }
   }
@@ -315,10 +322,10 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_long_weights_kernel(const 
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const reg_vec<T, VEC> vx = load_vec<T, VEC>(static_cast<const T*>(a.x) + row * a.x_stride + col, a.cols - col);
     const reg_vec<T, VEC> vd = load_vec<T, VEC>(static_cast<const T*>(a.dy) + row * a.dy_stride + col, a.cols - col);
-    const float mean = a.mean[row], r = a.rstd[row];
+    const float mean = a.mean[row], r = a.rstd[row], c = a.shift[row];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      dw[i] += vd[i] * ((vx[i] - mean) * r);
+      dw[i] += vd[i] * ((vx[i] - mean) * r - c);
       db[i] += vd[i];
     }
   }
@@ -394,8 +401,7 @@ static int launch_norm(const NormArgs& a, int64_t slots, void* stream) {
   if (a.cols > kNormKept) {
     const unsigned blocks = (unsigned)std::min<int64_t>(a.rows, 1024);
     if constexpr (!BWD) return launch(layer_norm_fwd_long_kernel<T, VEC>, dim3(blocks), dim3(1024), 0, stream, a);
-    int err = 0;
-    if (a.dx) err = launch(layer_norm_bwd_long_kernel<T, VEC>, dim3(blocks), dim3(1024), 0, stream, a);
+    int err = launch(layer_norm_bwd_long_kernel<T, VEC>, dim3(blocks), dim3(1024), 0, stream, a);
     if (err == 0 && a.part)
       err = launch(layer_norm_bwd_long_weights_kernel<T, VEC>, dim3((unsigned)((a.cols + 256 * VEC - 1) / (256 * VEC)), (unsigned)slots),
                    dim3(256), 0, stream, a);
@@ -452,7 +458,9 @@ extern "C" int socmx_layer_norm_fwd(int32_t type, int32_t wtype, const void* x, 
 
 extern "C" int64_t socmx_layer_norm_bwd_workspace_floats(int32_t type, int64_t rows, int64_t cols) {
   if (norm_check(type, type, rows, cols)) return 0;
-  return norm_slots(rows, (int)cols, type == SOCMX_F32 ? 4 : 8) * 2 * cols;
+  // (long rows: a float for each of them behind the slots, in whole slots)
+  const int64_t more = cols > kNormKept ? (rows + 2 * cols - 1) / (2 * cols) : 0;
+  return (norm_slots(rows, (int)cols, type == SOCMX_F32 ? 4 : 8) + more) * 2 * cols;
 }
 
 extern "C" int socmx_layer_norm_bwd(int32_t type, int32_t wtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
@@ -467,6 +475,7 @@ extern "C" int socmx_layer_norm_bwd(int32_t type, int32_t wtype, const void* x, 
   a.part = dweight || dbias ? workspace : nullptr;
   a.rows = rows; a.cols = (int)cols; a.x_stride = x_stride; a.dy_stride = dy_stride; a.w32 = wtype == SOCMX_F32;
   const int64_t slots = norm_slots(rows, (int)cols, type == SOCMX_F32 ? 4 : 8);
+  if (a.part && cols > kNormKept) a.shift = a.part + slots * 2 * cols;
   int err = dispatch_norm<true>(type, a, slots, stream);
   if (err || !a.part) return err;
   const dim3 grid((unsigned)((2 * cols + 31) / 32)), block(1024);

@@ -205,3 +205,50 @@ def test_a_second_derivative_is_refused_on_every_way_to_the_inputs():
     ref = torch.autograd.grad(layers.gated_scan(far(base), far(decay), init)[0].square().sum(), [base, decay, init])
     far_dense = torch.autograd.grad(layers.gated_scan(far(base).contiguous(), far(decay).contiguous(), init)[0].square().sum(), [base, decay, init])
     assert all(torch.equal(p, q) for p, q in zip(ref, far_dense))
+
+
+def far_rows_oracle(x, w, b, eps, dy):
+    """Outputs in 64 bits with their tolerances' float32 parts, for rows far from zero that hardly vary.
+
+    Nothing here scales with |mean| / deviation in the first order.  With m the float32 next to the mean (off by E <= k U mean|x|, k additions one
+    after the other), x - m is exact (x and m within a factor of 2), the mean of x - m is formed with an error of k U mean|x - m|, where
+    mean|x - m| <= mean|x - mu| + E; what is left of a variance shifted by E^2 is off by (k + 2) U (var + E^2)."""
+    x, dy, w, b = (t.double() for t in (x, dy, w, b))
+    D, R = x.shape[1], x.shape[0]
+    mu = x.mean(1, keepdim=True)
+    var = (x - mu).square().mean(1, keepdim=True)
+    r = 1 / (var + eps).sqrt()
+    n = (x - mu) * r
+    g = dy * w
+    s, q = g.mean(1, keepdim=True), (g * n).mean(1, keepdim=True)
+    dx = r * (g - s - n * q)
+    k = 32 + D / 1024
+    E = k * U * x.abs().mean(1, keepdim=True)
+    shift = 1 + E * E * r * r
+    dn = U * (k * r * ((x - mu).abs().mean(1, keepdim=True) + E) + (2 * k * shift + 8) * n.abs() + 2 * r * E)
+    tol_y = w.abs() * dn + 4 * U * ((n * w).abs() + b.abs())
+    G, GN = g.abs().mean(1, keepdim=True), (g * n).abs().mean(1, keepdim=True)
+    # the sums of g (n + c) and of g, c the part of the mean that is taken off afterwards, |c| <= E r
+    dq = (g.abs() * dn).mean(1, keepdim=True) + (k + 2) * U * (GN + E * r * G)
+    tol_dx = r * (4 * U * g.abs() + (k + 2) * U * G + n.abs() * dq + dn * q.abs() + 4 * U * (n * q).abs() + (2 * k * shift + 8) * U * (g - s - n * q).abs())
+    m = 64 + R / 256
+    return [(n * w + b, tol_y), (dx, tol_dx), ((dy * n).sum(0), (dy.abs() * dn).sum(0) + m * U * (dy * n).abs().sum(0)),
+            (dy.sum(0), m * U * dy.abs().sum(0))]
+
+
+@pytest.mark.parametrize("offset,spread", [(100.0, 1e-3), (1000.0, 1e-2), (-3e4, 1.0)])
+@pytest.mark.parametrize("rows,cols", [(40, 24), (40, 256), (30, 500), (40, 1601), (20, 4100), (6, 16384), (5, 20001)])
+def test_layer_norm_of_rows_that_hardly_vary(offset, spread, rows, cols):
+    """The part of the mean that one float32 does not hold, the same for a whole row, is in no output and no gradient."""
+    g = gen(rows + cols)
+    x = offset + spread * torch.randn(rows, cols, generator=g)
+    w, b = 1 + 0.3 * torch.randn(cols, generator=g), torch.randn(cols, generator=g)
+    dy = 1 + torch.randn(rows, cols, generator=g)
+    ts = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    y = layers.layer_norm(*ts)
+    got = [y] + list(torch.autograd.grad(y, ts, dy.to(DEV)))
+    for t, (want, tol) in zip(got, far_rows_oracle(x, w, b, 1e-5, dy)):
+        close(t, want, tol + half(F32) * want.abs() + tiny(F32))
+    for i in (1, 2):                                           # each gradient alone: the same bits
+        alone = [t.detach().requires_grad_(j == i - 1) for j, t in enumerate(ts)]
+        assert torch.equal(torch.autograd.grad(layers.layer_norm(*alone), alone[i - 1], dy.to(DEV))[0], got[i])
