@@ -48,7 +48,7 @@ struct AdamwArgs {
   int32_t count;
   const float* correction;           // (count, 4): lr / (1 - b1^t), 1 / sqrt(1 - b2^t), t (as an integer), unused
   double b1, b2;
-  float decay, eps;
+  float decay, eps;                  // decay: lr wd
 };
 
 struct AdamwValuesArgs {
@@ -107,7 +107,10 @@ __device__ __forceinline__ float adamw_weight(float p, float m, float v, float s
   } else {
     deviation = __builtin_amdgcn_sqrtf(v);
   }
-  float w = p * decay - size * m * __builtin_amdgcn_rcpf(deviation * root + eps);
+  // (What is taken off is formed first: a factor 1 - lr wd in f32 would be off by up to 2^-25, a fifth of a decay of 1e-7 and all of a smaller
+  // one.  An infinite weight stays one.)
+  const float held = __builtin_amdgcn_fmed3f(p, -3.40282347e38f, 3.40282347e38f);
+  float w = p - fmaf(held, decay, size * m * __builtin_amdgcn_rcpf(deviation * root + eps));
   asm("" : "+v"(w));      // a float32 from here on: a 16-bit weight is its rounding, not a second result of one mixed instruction
   return w;
 }
@@ -431,7 +434,7 @@ static int adamw_update(int32_t type, int32_t bits, const socmx_adamw_tensor* te
   int at = 0;
   while (at < ntensors) {
     AdamwArgs a;
-    a.b1 = beta1; a.b2 = beta2; a.decay = (float)(1.0 - lr * weight_decay); a.eps = (float)eps;
+    a.b1 = beta1; a.b2 = beta2; a.decay = (float)(lr * weight_decay); a.eps = (float)eps;
     a.correction = workspace + 4 * (int64_t)at;
     int64_t blocks = 0;
     int count = 0;

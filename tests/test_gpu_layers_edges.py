@@ -252,3 +252,32 @@ def test_layer_norm_of_rows_that_hardly_vary(offset, spread, rows, cols):
     for i in (1, 2):                                           # each gradient alone: the same bits
         alone = [t.detach().requires_grad_(j == i - 1) for j, t in enumerate(ts)]
         assert torch.equal(torch.autograd.grad(layers.layer_norm(*alone), alone[i - 1], dy.to(DEV))[0], got[i])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("kind,master", [(F32, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("lr,decay", [(1e-5, 1e-2), (1e-3, 5e-5), (1e-4, 4e-4), (3e-4, 1e-2)])
+def test_adamw_decay_of_a_small_share(bits, kind, master, lr, decay):
+    """lr wd far below 1, no gradient: the float32 weight is p - lr wd p with ONE rounding, half a step of the weight, and what the product
+    lr wd p is off by, 2 U of itself.  (A factor 1 - lr wd in float32 is off by up to 2^-25: a fifth of a decay of 1e-7.)"""
+    g = gen(41)
+    p = (1 + torch.rand(3000, generator=g)).to(kind)
+    w = p.float() + (2 ** -10 * torch.rand(3000, generator=g) if master else 0)
+    ps, ws = p.to(DEV), w.to(DEV)
+    m, v, scales, _ = new_states([3000], kind, bits, False, [ps])
+    optim.adamw_step([ps], [torch.zeros_like(ps)], m, v, torch.zeros(1, device=DEV), lr=lr, weight_decay=decay, scales=scales,
+                     masters=[ws] if master else None)
+    want = w.double() * (1 - lr * decay)
+    step = 2.0 ** (torch.floor(torch.log2(want)) - 24)         # half the distance of float32 numbers there
+    close(ws if master else ps, want, step + 2 * U * lr * decay * w.double() + 1e-15)
+    if master:
+        assert torch.equal(ps, ws.to(kind))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+def test_adamw_leaves_infinite_weights_infinite(bits, decay):
+    p = torch.tensor([math.inf, -math.inf, 1.0, math.nan], device=DEV)
+    m, v, scales, _ = new_states([4], F32, bits, False, [p])
+    optim.adamw_step([p], [torch.full((4,), 0.5, device=DEV)], m, v, torch.zeros(1, device=DEV), lr=1e-2, weight_decay=decay, scales=scales)
+    assert float(p[0]) == math.inf and float(p[1]) == -math.inf and 0.9 < float(p[2]) < 1.0 and math.isnan(float(p[3]))
