@@ -385,6 +385,22 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const May
   return {out[0], out[1]};
 }
 
+// whether a dense row of `s` (rows apart) and a dense row of `t` (rows at any distance) have memory in common
+bool rows_meet(const Tensor& s, const Tensor& t) {
+  if (s.numel() == 0 || t.numel() == 0) return false;
+  const int64_t s_size = s.size(1) * s.element_size(), t_size = t.size(1) * t.element_size(), s_step = s.stride(0) * s.element_size();
+  const int64_t t_step = t.stride(0) * t.element_size(), last = t.size(0) - 1;
+  const int64_t gap = static_cast<const char*>(s.data_ptr()) - static_cast<const char*>(t.data_ptr());      // from t's first byte to s's
+  if (gap >= last * t_step + t_size || -gap >= (s.size(0) - 1) * s_step + s_size) return false;
+  for (int64_t i = 0; i < s.size(0); ++i) {
+    const int64_t lo = gap + i * s_step, hi = lo + s_size;      // row i of s, in bytes behind t's first one
+    // t's row j begins at j t_step: the first one that ends behind lo
+    const int64_t j = t_step == 0 || lo < t_size ? 0 : (lo - t_size) / t_step + 1;
+    if (j <= last && j * t_step < hi && j * t_step + t_size > lo) return true;
+  }
+  return false;
+}
+
 Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) {
   const char* what = "gated_scan_step";
   not_traced(what);
@@ -398,6 +414,8 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
   if (state.requires_grad()) refuse(what, ": state is updated in place and must not require a gradient");
   if (B > 1 && state.stride(0) < D) refuse(what, ": the rows of state overlap (stride ", state.stride(0), ")");
   const Tensor x = dense_last(x0), a = dense_last(a0);
+  for (const Tensor* t : {&x, &a})
+    if (rows_meet(state, *t)) refuse(what, ": state shares memory with x or log_decay");
   Tensor h = empty({B, D}, x.scalar_type(), x.device());
   if (B) {
     const Launch l(x.device());

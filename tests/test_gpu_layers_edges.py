@@ -281,3 +281,26 @@ def test_adamw_leaves_infinite_weights_infinite(bits, decay):
     m, v, scales, _ = new_states([4], F32, bits, False, [p])
     optim.adamw_step([p], [torch.full((4,), 0.5, device=DEV)], m, v, torch.zeros(1, device=DEV), lr=1e-2, weight_decay=decay, scales=scales)
     assert float(p[0]) == math.inf and float(p[1]) == -math.inf and 0.9 < float(p[2]) < 1.0 and math.isnan(float(p[3]))
+
+
+def test_gated_scan_step_refuses_a_state_that_shares_memory():
+    """Elements that are read while others write them would be a race."""
+    x, a = torch.randn(3, 8, device=DEV), -torch.rand(3, 2, device=DEV)
+    wide = torch.zeros(3, 40, device=DEV)
+    state = wide[:, 4:12]
+    flat = wide.view(-1)
+    meet = lambda x, a: pytest.raises(SocmxError, match="shares memory")   # noqa: E731
+    for xs, As in ((state, a), (wide[:, 5:13], a), (wide[:, :8], a), (wide[:, 11:19], a), (x, wide[:, 2:6]), (x, wide[:, 11:13]),
+                   (flat[51:59].expand(3, 8), a), (flat[44:52].expand(3, 8), a), (x, flat[91:92].expand(3, 1)), (flat.as_strided((3, 8), (9, 1), 77), a),
+                   (wide.view(F16).as_strided((3, 8), (16, 1), 1), a), (x, flat[4:].as_strided((3, 8), (0, 1)))):
+        with meet(xs, As):
+            layers.gated_scan_step(state, xs, As)
+    assert not bool(wide.any())
+    wide[:, 12:20], wide[:, 2:4] = x, a
+    h = layers.gated_scan_step(state, wide[:, 12:20], wide[:, 2:4])          # (between each other in one buffer, and apart)
+    assert torch.equal(h, x) and torch.equal(wide[:, 4:12], x) and torch.equal(wide[:, 2:4], a) and not bool(wide[:, :2].any())
+    one = torch.zeros(30, device=DEV)
+    layers.gated_scan_step(one[:24].view(3, 8), one[24:].as_strided((3, 1), (1, 1)).expand(3, 8).contiguous(), one[24:27].view(3, 1))
+    layers.gated_scan_step(one[6:30].view(3, 8), one[:6].view(3, 2).repeat_interleave(4, 1), one[:6].view(3, 2))
+    layers.gated_scan_step(one[6:30].view(3, 8), one[:6].expand(3, 6).repeat(1, 2)[:, :8], one[5:6].expand(3, 1))
+    layers.gated_scan_step(wide[:2, 4:12], flat[52:60].expand(2, 8), a[:2])
