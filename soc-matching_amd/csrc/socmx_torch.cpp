@@ -405,6 +405,7 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
   const char* what = "gated_scan_step";
   not_traced(what);
   no_tangent(what, {&state, &x0, &a0});
+  const bool wants_grad = at::GradMode::is_enabled() && (x0.requires_grad() || a0.requires_grad());
   const at::NoGradGuard off;
   check_scan(what, x0, a0, 2);
   beside(what, x0, state);
@@ -413,6 +414,7 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
     refuse(what, ": state is (", B, ", ", D, ") float32 with dense rows, got ", shape(state), " ", state.scalar_type(), " strides ", state.strides());
   if (state.requires_grad()) refuse(what, ": state is updated in place and must not require a gradient");
   if (B > 1 && state.stride(0) < D) refuse(what, ": the rows of state overlap (stride ", state.stride(0), ")");
+  if (wants_grad) refuse(what, ": x or log_decay requires a gradient, and a step has none: detach them or take the step under no_grad");
   const Tensor x = dense_last(x0), a = dense_last(a0);
   for (const Tensor* t : {&x, &a})
     if (rows_meet(state, *t)) refuse(what, ": state shares memory with x or log_decay");

@@ -64,5 +64,6 @@ def gated_scan(x, log_decay, initial=None, lengths=None, reverse=False):
 
 def gated_scan_step(state, x, log_decay):
     """One step of `gated_scan` while a control is evaluated: state (B, D) float32 becomes exp(log_decay) state + x IN PLACE; returns it
-    rounded to x's type, (B, D).  x (B, D), log_decay (B, G), neither in state's memory.  Not differentiable."""
+    rounded to x's type, (B, D).  x (B, D), log_decay (B, G), neither in state's memory.  Not differentiable: inputs that require a gradient are
+    refused where gradients are recorded."""
     return _binding().gated_scan_step(state, x, log_decay)

@@ -304,3 +304,16 @@ def test_gated_scan_step_refuses_a_state_that_shares_memory():
     layers.gated_scan_step(one[6:30].view(3, 8), one[:6].view(3, 2).repeat_interleave(4, 1), one[:6].view(3, 2))
     layers.gated_scan_step(one[6:30].view(3, 8), one[:6].expand(3, 6).repeat(1, 2)[:, :8], one[5:6].expand(3, 1))
     layers.gated_scan_step(wide[:2, 4:12], flat[52:60].expand(2, 8), a[:2])
+
+
+def test_gated_scan_step_refuses_inputs_that_want_a_gradient():
+    """It is not dropped without a word."""
+    x, a = torch.randn(3, 8, device=DEV), -torch.rand(3, 2, device=DEV)
+    for ts in ((x.clone().requires_grad_(), a), (x, a.clone().requires_grad_())):
+        state = torch.zeros(3, 8, device=DEV)
+        with pytest.raises(SocmxError, match="gradient"):
+            layers.gated_scan_step(state, *ts)
+        assert not bool(state.any())
+        with torch.no_grad():
+            layers.gated_scan_step(state, *ts)
+        assert torch.equal(state, x)
