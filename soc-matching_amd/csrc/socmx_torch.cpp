@@ -431,6 +431,25 @@ Tensor gated_scan_step(const Tensor& state, const Tensor& x0, const Tensor& a0) 
 
 // ---- AdamW -------------------------------------------------------------------------------------------------------------------------
 typedef std::vector<Tensor> Tensors;
+
+struct Span {                                // the memory of a dense tensor
+  uintptr_t begin;
+  uint64_t bytes : 63, written : 1;
+  Span(const void* p, uint64_t size, bool w) : begin(reinterpret_cast<uintptr_t>(p)), bytes(size), written(w) {}
+};
+
+// whether any of them that is written shares memory with another one
+bool shared(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t any = 0, written = 0;            // how far those in front reach
+  for (const Span& s : spans) {
+    if (s.begin < (s.written ? any : written)) return true;
+    any = std::max<uintptr_t>(any, s.begin + s.bytes);
+    if (s.written) written = std::max<uintptr_t>(written, s.begin + s.bytes);
+  }
+  return false;
+}
+
 constexpr int64_t kBlock = 256;
 
 // steps: one tensor with a count for each of the params, or `counts`: a tensor of one element for each
@@ -458,8 +477,9 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
   for (size_t i = 0; i < count; ++i) no_tangent(what, {&params[i], &grads[i], &ms[i], &vs[i]});
   std::vector<socmx_adamw_tensor> rows(count);
-  std::vector<const void*> written_to;
-  written_to.reserve(6 * count);
+  const int64_t bytes = params[0].element_size();
+  std::vector<Span> spans;
+  spans.reserve(7 * count + 1);
   std::vector<float*> at;
   if (counts)
     for (size_t i = 0; i < count; ++i) {
@@ -467,8 +487,10 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
       if (t.numel() != 1 || t.scalar_type() != at::kFloat || t.device() != dev)
         refuse(what, ": the step count of tensor ", i, " is one float32 on ", dev, ", got ", shape(t), " ", t.scalar_type(), " on ", t.device());
       at.push_back(t.data_ptr<float>());
-      written_to.push_back(at.back());
+      spans.emplace_back(at.back(), 4, true);
     }
+  else
+    spans.emplace_back(pointer(steps), 4 * count, true);
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = ms[i], &v = vs[i];
     const Tensor s = scales ? (*scales)[i] : Tensor(), w = masters ? (*masters)[i] : Tensor();
@@ -483,14 +505,18 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
     for (const Tensor* t : {&p, &g, &m, &v, &s, &w})
       if (t->defined() && (t->device() != dev || !t->is_contiguous()))
         refuse(what, ": tensor ", i, " has a part on ", t->device(), " with strides ", t->strides(), "; dense ones on ", dev, " are needed");
-    if (n)
-      for (const Tensor* t : {&p, &m, &v, &s, &w})
-        if (t->defined()) written_to.push_back(t->data_ptr());
     rows[i] = socmx_adamw_tensor{pointer(p), pointer(g), pointer(m), pointer(v), pointer_as<float>(s), pointer_as<float>(w), n};
+    if (n) {
+      const int64_t state = n * (scales ? 1 : 4);
+      spans.emplace_back(rows[i].p, n * bytes, true);
+      spans.emplace_back(rows[i].grad, n * bytes, false);
+      spans.emplace_back(rows[i].exp_avg, state, true);
+      spans.emplace_back(rows[i].exp_avg_sq, state, true);
+      if (scales) spans.emplace_back(rows[i].scale, 8 * s.size(0), true);
+      if (masters) spans.emplace_back(rows[i].master, 4 * n, true);
+    }
   }
-  std::sort(written_to.begin(), written_to.end());
-  if (std::adjacent_find(written_to.begin(), written_to.end()) != written_to.end())
-    refuse(what, ": one of the tensors, states or masters is another tensor's too");
+  if (shared(spans)) refuse(what, ": memory of one of the tensors, states, masters or counts is another tensor's too (gradients may be shared among themselves)");
   const Tensor ws = floats(4 * (int64_t)count, dev);
   const Launch l(dev);
   const int type_id = element_type(params[0]), bits = scales ? 8 : 32;

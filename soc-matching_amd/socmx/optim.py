@@ -27,7 +27,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     tensors of the same sizes; with `scales`, 8-bit states: int8 and uint8 codes and a float32 (ceil(n / 256), 2) for each tensor of n
     elements (zeros are states of zero; `adamw_state_values` decodes).  masters: float32 weights the update works on, the 16-bit
     weights getting their rounding.  steps: (len(params),) float32 on the GPU, or a list of tensors of one float32 each: the updates so
-    far, advanced here -- a captured call counts its replays.  No two tensors may share memory; a tensor may be empty."""
+    far, advanced here -- a captured call counts its replays.  No two tensors may share memory, but gradients among themselves; a
+    tensor may be empty."""
     if torch.is_tensor(lr):
         raise SocmxError("adamw_step: lr is a number, got a tensor")
     binding = _lib.torch_binding()

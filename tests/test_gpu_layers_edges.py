@@ -317,3 +317,37 @@ def test_gated_scan_step_refuses_inputs_that_want_a_gradient():
         with torch.no_grad():
             layers.gated_scan_step(state, *ts)
         assert torch.equal(state, x)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_memory_that_is_shared_in_part(bits):
+    """Not the same first element only: any element that one tensor's update writes and another's reads or writes."""
+    n = 600
+    flat = torch.zeros(4 * n, device=DEV)
+    f = lambda t=F32: torch.zeros(n, dtype=t, device=DEV)   # noqa: E731
+    kinds = (F32, F32) if bits == 32 else (torch.int8, torch.uint8)
+
+    def call(**kw):
+        a = dict(params=[f(), f()], grads=[f(), f()], exp_avgs=[f(kinds[0]), f(kinds[0])], exp_avg_sqs=[f(kinds[1]), f(kinds[1])],
+                 steps=torch.zeros(2, device=DEV), lr=1e-3)
+        if bits == 8:
+            a["scales"] = [torch.zeros(optim.scale_rows(n), 2, device=DEV) for _ in range(2)]
+        optim.adamw_step(**{**a, **kw})
+    call(params=[flat[:n], flat[n:2 * n]], grads=[flat[2 * n:3 * n], flat[2 * n + 1:3 * n + 1]])      # (gradients may overlap each other)
+    small = torch.zeros(n, dtype=kinds[0], device=DEV)
+    for bad in (dict(params=[flat[:n], flat[n - 1:2 * n - 1]]), dict(params=[flat[:n], f()], grads=[f(), flat[1:n + 1]]),
+                dict(params=[flat[:n], f()], grads=[flat[:n], f()]), dict(params=[f(), flat[1:n + 1]], grads=[flat[:n], f()]),
+                dict(params=[flat[:n], f()], steps=flat[n - 1:n + 1]), dict(grads=[flat[:n], f()], steps=flat[n - 1:n + 1]),
+                dict(grads=[flat[:n], f()], steps=[flat[4], flat[3 * n]]), dict(exp_avgs=[small, small]),
+                dict(steps=[flat[3], flat[3]])):
+        with pytest.raises(SocmxError, match="another tensor's"):
+            call(**bad)
+    if bits == 8:
+        scales = torch.zeros(2 * optim.scale_rows(n), 2, device=DEV)
+        call(scales=[scales[:optim.scale_rows(n)], scales[optim.scale_rows(n):]])
+        with pytest.raises(SocmxError, match="another tensor's"):
+            call(scales=[scales[:optim.scale_rows(n)], scales[1:1 + optim.scale_rows(n)]])
+        codes = torch.zeros(2 * n, dtype=torch.int8, device=DEV)
+        with pytest.raises(SocmxError, match="another tensor's"):
+            call(exp_avgs=[codes[:n], codes[n - 1:2 * n - 1]])
+    assert not bool(flat.any())
