@@ -613,7 +613,8 @@ int socmx_gated_scan_step(int32_t type, int32_t gate_type, int32_t B, int32_t D,
  *   exp_avg_sq uint8 codes with scale (ceil(n / 256), 2) f32, m = scale0 c |c| / 127^2, v = scale1 (c / 255)^4 (csrc/socmx_adamw.hip);
  *   codes and scales 0 are states of 0.  socmx_adamw_state_values writes what codes stand for, in f32.
  * steps (ntensors,) f32 device: the updates each tensor has had, advanced by the call (so that a captured call counts its replays).
- * workspace: 4 ntensors floats.  No two tensors may overlap; n may be 0 (the step is counted).
+ * workspace: 4 ntensors floats.  No two tensors may overlap; n may be 0 (the step is counted) and at most 4096 (2^24 - 1), else SOCMX_E_DIM and
+ *   nothing is launched.
  * socmx_adamw_step_counts: the same with each tensor's count where it lies (steps: HOST array of ntensors device pointers, read during the
  *   call), so that a tensor's count keeps its address whichever others are updated with it.
  */

@@ -396,6 +396,8 @@ __global__ __launch_bounds__(256) void adamw8_values_kernel(const AdamwValuesArg
 }
 
 static inline int64_t adamw_chunks(int64_t n) { return (n + kAdamwChunk - 1) / kAdamwChunk; }
+// the workgroups of a launch, whose threads are counted in 32 bits (a tensor of them all: 2^36 elements)
+constexpr int64_t kAdamwGroups = UINT32_MAX / 256;
 
 }  // namespace socmx
 
@@ -410,7 +412,7 @@ static int adamw_update(int32_t type, int32_t bits, const socmx_adamw_tensor* te
   for (int i = 0; i < ntensors; ++i) {
     const socmx_adamw_tensor& t = tensors[i];
     if (counts && !counts[i]) return SOCMX_E_NULL;
-    if (t.n < 0 || t.n > (1ll << 40)) return SOCMX_E_DIM;
+    if (t.n < 0 || t.n > kAdamwGroups * kAdamwChunk) return SOCMX_E_DIM;
     if (t.n == 0) continue;
     if (!t.p || !t.grad || !t.exp_avg || !t.exp_avg_sq || (bits == 8 && !t.scale)) return SOCMX_E_NULL;
     if (t.master && type == SOCMX_F32) return SOCMX_E_KIND;
@@ -441,8 +443,7 @@ static int adamw_update(int32_t type, int32_t bits, const socmx_adamw_tensor* te
     for (; count < kAdamwTensors && at + count < ntensors; ++count) {
       const socmx_adamw_tensor& t = tensors[at + count];
       const int64_t more = adamw_chunks(t.n);
-      if (more > 0x3FFFFFFF) return SOCMX_E_DIM;
-      if (blocks + more > 0x7FFFFFFF) break;
+      if (blocks + more > kAdamwGroups) break;
       a.tensor[count] = AdamwTensor{t.p, t.grad, t.exp_avg, t.exp_avg_sq, t.scale, t.master, t.n};
       a.first[count] = (int32_t)blocks;
       blocks += more;
@@ -482,7 +483,7 @@ extern "C" int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t
   if (nstates < 1) return SOCMX_E_DIM;
   for (int i = 0; i < nstates; ++i) {
     const socmx_adamw_state& t = states[i];
-    if (t.n < 1 || t.n > (1ll << 40)) return SOCMX_E_DIM;
+    if (t.n < 1 || t.n > kAdamwGroups * kAdamwChunk) return SOCMX_E_DIM;
     if (!t.exp_avg || !t.exp_avg_sq || !t.scale || !t.out_exp_avg || !t.out_exp_avg_sq) return SOCMX_E_NULL;
   }
   int at = 0;
@@ -493,7 +494,7 @@ extern "C" int socmx_adamw_state_values(const socmx_adamw_state* states, int32_t
     for (; count < kAdamwTensors && at + count < nstates; ++count) {
       const socmx_adamw_state& t = states[at + count];
       const int64_t more = adamw_chunks(t.n);
-      if (blocks + more > 0x7FFFFFFF) break;
+      if (blocks + more > kAdamwGroups) break;
       a.m[count] = t.exp_avg; a.v[count] = t.exp_avg_sq; a.scale[count] = t.scale;
       a.out_m[count] = t.out_exp_avg; a.out_v[count] = t.out_exp_avg_sq; a.n[count] = t.n;
       a.first[count] = (int32_t)blocks;

@@ -85,3 +85,13 @@ def test_tracing_is_refused():
             torch.jit.trace(f, args, check_trace=False)
         with pytest.raises(SocmxError, match="cannot be traced"):
             make_fx(f)(*args)
+
+
+def test_adamw_refuses_what_a_launch_cannot_count():
+    """A launch counts its threads in 32 bits: 2^24 - 1 workgroups of 256, 4096 elements each.  Refused before anything is launched."""
+    L = _lib.lib()
+    hyper = (1e-3, 0.9, 0.999, 1e-8, 0.01)
+    most = 4096 * (2 ** 24 - 1)
+    for n in (most + 1, 2 ** 37, 2 ** 40, 2 ** 62):
+        assert L.socmx_adamw_step(0, 32, _adamw([(1, 1, 1, 1, 1, 0, 5), (1, 1, 1, 1, 1, 0, n)]), 2, 1, 1, *hyper, None) == -2
+        assert L.socmx_adamw_state_values(_adamw([(1, 1, 1, 1, 1, n)]), 1, None) == -2
