@@ -293,9 +293,13 @@ socmx_scan descriptor(const Tensor& x, const Tensor& a, const Tensor& lengths, b
   return s;
 }
 
+// no step, or no row: the state is what it was
+bool no_steps(const Tensor& x) { return x.size(0) == 0 || x.size(1) == 0; }
+
 std::pair<Tensor, Tensor> scan_forward(const Tensor& x, const Tensor& a, const Tensor& initial, const Tensor& lengths, bool reverse,
                                        Tensor* states) {
   const at::Device dev = x.device();
+  if (no_steps(x)) return {laid_like(x), initial.defined() ? initial.clone() : at::zeros({x.size(1), x.size(2)}, x.options().dtype(at::kFloat).requires_grad(false))};
   const socmx_scan s = descriptor(x, a, lengths, reverse);
   int64_t n_states, n_ws, n_bwd;
   check(abi.socmx_gated_scan_sizes(&s, &n_states, &n_ws, &n_bwd), "socmx_gated_scan_sizes");
@@ -327,13 +331,19 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &a = saved[1], &states = saved[2], &lengths = saved[3];
     const at::Device dev = x.device();
+    const bool need_initial = ctx->saved_data["initial"].toBool() && ctx->needs_input_grad(2);
+    Tensor dx = laid_like(x), da = laid_like(a), dinitial;
+    if (need_initial) dinitial = empty({x.size(1), x.size(2)}, at::kFloat, dev);
+    if (no_steps(x)) {
+      if (need_initial && grads[1].defined()) dinitial.copy_(grads[1]);
+      else if (need_initial) dinitial.zero_();
+      return once("gated_scan", {dx, da, dinitial, Tensor(), Tensor()}, grads);
+    }
     const socmx_scan s = descriptor(x, a, lengths, ctx->saved_data["reverse"].toBool());
     int64_t n_states, n_fwd, n_ws;
     check(abi.socmx_gated_scan_sizes(&s, &n_states, &n_fwd, &n_ws), "socmx_gated_scan_sizes");
     const Tensor ws = floats(n_ws, dev);
     const Tensor dh = grads[0].defined() ? dense_last(grads[0]) : Tensor(), dfinal = grads[1].defined() ? grads[1].contiguous() : Tensor();
-    Tensor dx = laid_like(x), da = laid_like(a), dinitial;
-    if (ctx->saved_data["initial"].toBool() && ctx->needs_input_grad(2)) dinitial = empty({x.size(1), x.size(2)}, at::kFloat, dev);
     {
       const Launch l(dev);
       check(abi.socmx_gated_scan_bwd(&s, pointer(x), pointer(a), states.data_ptr<float>(), pointer(dh), dh.defined() ? dh.stride(0) : 0,
@@ -366,15 +376,13 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& a, const May
   not_traced(what);
   no_tangent(what, {&x, &a, given(initial)});
   check_scan(what, x, a, 3);
-  const int64_t T = x.size(0), B = x.size(1), D = x.size(2);
+  const int64_t B = x.size(1), D = x.size(2);
   beside(what, x, initial);
   beside(what, x, lengths);
   if (initial && (initial->dim() != 2 || initial->size(0) != B || initial->size(1) != D || initial->scalar_type() != at::kFloat))
     refuse(what, ": initial is (", B, ", ", D, ") float32, got ", shape(*initial), " ", initial->scalar_type());
   if (lengths && (lengths->dim() != 1 || lengths->size(0) != B || lengths->scalar_type() != at::kInt))
     refuse(what, ": lengths is (", B, ",) int32, got ", shape(*lengths), " ", lengths->scalar_type());
-  if (T == 0 || B == 0)     // no step, or no row: the state is what it was
-    return {x + 0, initial ? *initial + 0 : at::zeros({B, D}, x.options().dtype(at::kFloat))};
   const Tensor first = initial.value_or(Tensor()), n = lengths ? lengths->contiguous() : Tensor();
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || a.requires_grad() || (initial && first.requires_grad()))) {
     at::NoGradGuard off;

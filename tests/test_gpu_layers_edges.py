@@ -351,3 +351,18 @@ def test_adamw_refuses_memory_that_is_shared_in_part(bits):
         with pytest.raises(SocmxError, match="another tensor's"):
             call(exp_avgs=[codes[:n], codes[n - 1:2 * n - 1]])
     assert not bool(flat.any())
+
+
+@pytest.mark.parametrize("T,B", [(0, 3), (5, 0), (0, 0)])
+def test_gated_scan_gradients_of_no_steps_and_no_rows(T, B):
+    """Every input has a gradient: nothing for x and log_decay, the final state's for the initial one."""
+    x, a = torch.zeros(T, B, 4, device=DEV, requires_grad=True), torch.zeros(T, B, 2, device=DEV, requires_grad=True)
+    init = torch.ones(B, 4, device=DEV, requires_grad=True)
+    h, final = layers.gated_scan(x, a, init)
+    assert h.shape == (T, B, 4) and torch.equal(final, init) and (B == 0 or final.data_ptr() != init.data_ptr())
+    up = torch.arange(4 * B, device=DEV).reshape(B, 4).float()
+    gx, ga, g0 = torch.autograd.grad([h, final], [x, a, init], [torch.zeros_like(h), up])
+    assert gx.shape == x.shape and ga.shape == a.shape and torch.equal(g0, up)
+    h, final = layers.gated_scan(x, a)
+    gx, ga = torch.autograd.grad(h.sum() + final.sum(), [x, a])
+    assert gx.shape == x.shape and ga.shape == a.shape and final.shape == (B, 4) and not bool(final.any())
