@@ -77,8 +77,16 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def load_state_dict(self, state_dict):
-        """torch casts what it loads to the parameters' type: codes, masters and float32 states of 16-bit weights are taken as they are."""
+        """torch casts what it loads to the parameters' type: codes, masters and float32 states of 16-bit weights are taken as they are.
+        A state of torch.optim.AdamW is taken too, without its amsgrad and maximize, which are refused."""
+        for group in state_dict["param_groups"]:
+            for name in ("amsgrad", "maximize"):
+                if group.get(name):
+                    raise SocmxError(f"AdamW: a state with {name} cannot be continued")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             for name, v in state_dict["state"].get(i, {}).items():

@@ -366,3 +366,30 @@ def test_gated_scan_gradients_of_no_steps_and_no_rows(T, B):
     h, final = layers.gated_scan(x, a)
     gx, ga = torch.autograd.grad(h.sum() + final.sum(), [x, a])
     assert gx.shape == x.shape and ga.shape == a.shape and final.shape == (B, 4) and not bool(final.any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_goes_on_from_a_state_of_torch(bits):
+    """Parameters that torch has stepped go on in 32 bits, those that it has not get the new optimiser's states."""
+    g = gen(61)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=g).to(DEV)) for n in (300, 41)]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    kw = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-6, weight_decay=0.1)
+    ref = torch.optim.AdamW(ps, **kw)
+    for p in ps[:1]:
+        p.grad = torch.randn(p.shape, generator=g).to(DEV)
+    ref.step()
+    qs[0].data.copy_(ps[0])
+    opt = optim.AdamW(qs, state_bits=bits)
+    opt.load_state_dict(ref.state_dict())
+    for _ in range(3):
+        for p, q in zip(ps, qs):
+            p.grad = torch.randn(p.shape, generator=g).to(DEV)
+            q.grad = p.grad.clone()
+        ref.step()
+        opt.step()
+    # 24 roundings on either side of each update, none longer than 3 lr (the codes of the parameter that is new to both differ in 8 bits)
+    for p, q in zip(ps[:1 if bits == 8 else 2], qs):
+        close(q, p.detach(), 2 * 3 * U * (3 * p.detach().abs().double().cpu() + 24 * 3e-2))
+    assert [float(opt.state[q]["step"]) for q in qs] == [4.0, 3.0]
+    assert opt.state[qs[0]]["exp_avg"].dtype == F32 and ("scale" in opt.state[qs[1]]) == (bits == 8)

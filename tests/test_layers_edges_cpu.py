@@ -95,3 +95,25 @@ def test_adamw_refuses_what_a_launch_cannot_count():
     for n in (most + 1, 2 ** 37, 2 ** 40, 2 ** 62):
         assert L.socmx_adamw_step(0, 32, _adamw([(1, 1, 1, 1, 1, 0, 5), (1, 1, 1, 1, 1, 0, n)]), 2, 1, 1, *hyper, None) == -2
         assert L.socmx_adamw_state_values(_adamw([(1, 1, 1, 1, 1, n)]), 1, None) == -2
+
+
+def test_adamw_takes_a_state_of_torch():
+    """Its groups have no state_bits and no master_weights: the defaults of the optimiser that loads them.  What the rule does not have is refused."""
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (3, 4)]
+    params[0].grad = torch.ones(3)
+
+    def torch_state(**kw):
+        ref = torch.optim.AdamW(params, lr=1e-2, **kw)
+        ref.step()
+        return ref.state_dict()
+    for bits in (32, 8):
+        opt = optim.AdamW(params, lr=1e-3, state_bits=bits)
+        opt.load_state_dict(torch_state())
+        group, = opt.param_groups
+        assert group["lr"] == 1e-2 and group["state_bits"] == bits and group["master_weights"] is True
+        assert set(opt.state[params[0]]) == {"step", "exp_avg", "exp_avg_sq"} and params[1] not in opt.state
+    before = optim.AdamW(params, lr=1e-3)
+    for name in ("amsgrad", "maximize"):
+        with pytest.raises(SocmxError, match=name):
+            before.load_state_dict(torch_state(**{name: True}))
+    assert before.param_groups[0]["lr"] == 1e-3 and not before.state
