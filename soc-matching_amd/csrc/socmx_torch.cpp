@@ -510,9 +510,16 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
       refuse(what, ": the sizes of tensor ", i, " differ: ", n, " weights, ", g.numel(), " gradients, ", m.numel(), " and ", v.numel(), " states");
     if (scales && (s.dim() != 2 || s.size(0) != (n + kBlock - 1) / kBlock || s.size(1) != 2 || s.scalar_type() != at::kFloat))
       refuse(what, ": the scales of tensor ", i, " are (", (n + kBlock - 1) / kBlock, ", 2) float32, got ", shape(s), " ", s.scalar_type());
-    for (const Tensor* t : {&p, &g, &m, &v, &s, &w})
-      if (t->defined() && (t->device() != dev || !t->is_contiguous()))
-        refuse(what, ": tensor ", i, " has a part on ", t->device(), " with strides ", t->strides(), "; dense ones on ", dev, " are needed");
+    // (any order of the dimensions in memory, the same for all: the update goes by memory)
+    const bool plain = p.is_contiguous();
+    for (const Tensor* t : {&p, &g, &m, &v, &s, &w}) {
+      if (!t->defined()) continue;
+      const bool alike = plain || t == &s ? t->is_contiguous()
+                                          : t->is_non_overlapping_and_dense() && t->sizes() == p.sizes() && t->strides() == p.strides();
+      if (t->device() != dev || !alike)
+        refuse(what, ": tensor ", i, " has a part on ", t->device(), " with strides ", t->strides(), " beside ", p.strides(), "; dense ones on ", dev,
+               ", laid out alike, are needed");
+    }
     rows[i] = socmx_adamw_tensor{pointer(p), pointer(g), pointer(m), pointer(v), pointer_as<float>(s), pointer_as<float>(w), n};
     if (n) {
       const int64_t state = n * (scales ? 1 : 4);

@@ -23,8 +23,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
 
         m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
 
-    params, grads: lists of contiguous tensors of ONE type (float32, bfloat16 or float16) on one GPU.  exp_avgs, exp_avg_sqs: float32
-    tensors of the same sizes; with `scales`, 8-bit states: int8 and uint8 codes and a float32 (ceil(n / 256), 2) for each tensor of n
+    params, grads: lists of dense tensors of ONE type (float32, bfloat16 or float16) on one GPU, contiguous or, with all that belongs to a
+    parameter, of one other order of dimensions in memory.  exp_avgs, exp_avg_sqs: float32 tensors of the same sizes; with `scales`, 8-bit states: int8 and uint8 codes and a float32 (ceil(n / 256), 2) for each tensor of n
     elements (zeros are states of zero; `adamw_state_values` decodes).  masters: float32 weights the update works on, the 16-bit
     weights getting their rounding.  steps: (len(params),) float32 on the GPU, or a list of tensors of one float32 each: the updates so
     far, advanced here -- a captured call counts its replays.  No two tensors may share memory, but gradients among themselves; a
@@ -69,12 +69,18 @@ class AdamW(torch.optim.Optimizer):
         st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
         kinds = (torch.float32, torch.float32) if group["state_bits"] == 32 else (torch.int8, torch.uint8)
         for name, kind in zip(("exp_avg", "exp_avg_sq"), kinds):
-            st[name] = torch.zeros(p.shape, dtype=kind, device=p.device)
+            st[name] = torch.zeros_like(p, dtype=kind, requires_grad=False)          # (dense, in p's order of dimensions)
         if group["state_bits"] == 8:
             st["scale"] = torch.zeros(scale_rows(p.numel()), 2, dtype=torch.float32, device=p.device)
         if group["master_weights"] and p.dtype != torch.float32:
-            st["master"] = p.detach().to(torch.float32).contiguous()
+            st["master"] = p.detach().to(torch.float32)
         return st
+
+    @staticmethod
+    def _laid_like(grad, p):
+        if p.is_contiguous() and grad.is_contiguous() or grad.stride() == p.stride():
+            return grad
+        return torch.empty_like(p, requires_grad=False).copy_(grad)
 
     def load_state_dict(self, state_dict):
         """torch casts what it loads to the parameters' type: codes, masters and float32 states of 16-bit weights are taken as they are.
@@ -109,7 +115,7 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state.get(p) or self._new_state(p, group)
                 kinds.setdefault((p.dtype, p.device, "scale" in st, "master" in st), []).append((p, st))
             for (_, _, small, master), found in kinds.items():
-                adamw_step([p for p, _ in found], [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in found],
+                adamw_step([p for p, _ in found], [self._laid_like(p.grad, p) for p, _ in found],
                            [st["exp_avg"] for _, st in found], [st["exp_avg_sq"] for _, st in found], [st["step"] for _, st in found],
                            lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                            scales=[st["scale"] for _, st in found] if small else None,

@@ -393,3 +393,35 @@ def test_adamw_goes_on_from_a_state_of_torch(bits):
         close(q, p.detach(), 2 * 3 * U * (3 * p.detach().abs().double().cpu() + 24 * 3e-2))
     assert [float(opt.state[q]["step"]) for q in qs] == [4.0, 3.0]
     assert opt.state[qs[0]]["exp_avg"].dtype == F32 and ("scale" in opt.state[qs[1]]) == (bits == 8)
+
+
+@pytest.mark.parametrize("kind,bits", [(F32, 32), (F32, 8), (BF16, 8)])
+def test_adamw_of_parameters_in_other_orders_in_memory(kind, bits):
+    """A transposed weight and one with its channels last: the bits of the same memory as contiguous parameters, also with gradients laid out
+    differently, through a saved state, and in step."""
+    g = gen(71)
+    base = [torch.randn(17, 40, generator=g).to(kind).to(DEV), torch.randn(3, 5, 7, 4, generator=g).to(kind).to(DEV)]
+    turn = (lambda t: t.t(), lambda t: t.permute(0, 3, 1, 2))
+    make = lambda ps: optim.AdamW(ps, lr=1e-2, weight_decay=0.1, state_bits=bits)   # noqa: E731
+    plain = [torch.nn.Parameter(t.clone()) for t in base]
+    turned = [torch.nn.Parameter(f(t.clone())) for f, t in zip(turn, base)]
+    assert not any(p.is_contiguous() for p in turned)
+    a, b = make(plain), make(turned)
+    for k in range(4):
+        for f, p, q in zip(turn, plain, turned):
+            p.grad = torch.randn(p.shape, generator=g).to(kind).to(DEV)
+            q.grad = f(p.grad.clone()) if k % 2 else f(p.grad).contiguous()
+        a.step()
+        b.step()
+        if k == 1:
+            state = b.state_dict()
+            b = make(turned)
+            b.load_state_dict(state)
+    for f, p, q in zip(turn, plain, turned):
+        assert torch.equal(f(p), q)
+        for name, v in a.state[p].items():
+            assert torch.equal(f(v) if v.dim() > 2 or name in ("exp_avg", "exp_avg_sq", "master") else v, b.state[q][name]), name
+    t = lambda *s: torch.zeros(*s, device=DEV)   # noqa: E731
+    for p, q in ((t(4, 6).t(), t(6, 4)), (t(6, 4), t(4, 6).t()), (t(4, 12)[:, ::2], t(4, 6)), (t(4, 1).expand(4, 6), t(4, 6)), (t(4, 6).t(), t(24))):
+        with pytest.raises(SocmxError, match="laid out alike"):
+            optim.adamw_step([p], [q], [t(p.shape)], [t(p.shape)], t(1), lr=1e-3)
