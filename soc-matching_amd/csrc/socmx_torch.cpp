@@ -9,6 +9,7 @@
 #include <dlfcn.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
@@ -483,7 +484,8 @@ void adamw_update(const Tensors& params, const Tensors& grads, const Tensors& ms
   if (!counts && (steps.dim() != 1 || steps.size(0) != (int64_t)count || steps.scalar_type() != at::kFloat || steps.device() != dev || !steps.is_contiguous()))
     refuse(what, ": steps is a dense (", count, ",) float32 on ", dev, ", got ", shape(steps), " ", steps.scalar_type(), " on ", steps.device());
   const at::ScalarType mt = scales ? at::kChar : at::kFloat, vt = scales ? at::kByte : at::kFloat;
-  for (size_t i = 0; i < count; ++i) no_tangent(what, {&params[i], &grads[i], &ms[i], &vs[i]});
+  if (torch::autograd::ForwardADLevel::try_get_by_idx(0))          // (no level is open, no tensor has a tangent)
+    for (size_t i = 0; i < count; ++i) no_tangent(what, {&params[i], &grads[i], &ms[i], &vs[i]});
   std::vector<socmx_adamw_tensor> rows(count);
   const int64_t bytes = params[0].element_size();
   std::vector<Span> spans;

@@ -425,3 +425,14 @@ def test_adamw_of_parameters_in_other_orders_in_memory(kind, bits):
     for p, q in ((t(4, 6).t(), t(6, 4)), (t(6, 4), t(4, 6).t()), (t(4, 12)[:, ::2], t(4, 6)), (t(4, 1).expand(4, 6), t(4, 6)), (t(4, 6).t(), t(24))):
         with pytest.raises(SocmxError, match="laid out alike"):
             optim.adamw_step([p], [q], [t(p.shape)], [t(p.shape)], t(1), lr=1e-3)
+
+
+def test_adamw_refuses_tangents():
+    import torch.autograd.forward_ad as fwad
+    f = lambda: torch.ones(10, device=DEV)   # noqa: E731
+    ok = dict(params=[f()], grads=[f()], exp_avgs=[f()], exp_avg_sqs=[f()], steps=torch.zeros(1, device=DEV), lr=1e-3)
+    with fwad.dual_level(), torch.no_grad():
+        optim.adamw_step(**ok)
+        for name in ("params", "grads", "exp_avgs", "exp_avg_sqs"):
+            with pytest.raises(SocmxError, match="forward-mode"):
+                optim.adamw_step(**{**ok, name: [fwad.make_dual(f(), f())]})
