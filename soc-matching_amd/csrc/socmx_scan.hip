@@ -773,22 +773,23 @@ static int launch_scan(ScanArgs a, const ScanPlan& p, void* workspace, void* str
   }
   const dim3 grid((unsigned)(p.blocks * p.chunks)), block(64 * p.W);
   int err = SOCMX_E_DIM;               // (the forms that scan_plan never asks for are not compiled)
-  constexpr bool can_own = BWD ? V == 1 : (sizeof(T) + sizeof(TA)) * V <= 8, can_share = sizeof(T) * V <= 8;
+  // (a gate of 16 V channels leaves V at its widest)
+  constexpr bool can_own = BWD ? V == 1 : (sizeof(T) + sizeof(TA)) * V <= 8, can_share = sizeof(T) * V <= 8, can_row = sizeof(T) * V == 8;
   if constexpr (!BWD) {
     if constexpr (can_own)
       if (own) return launch(gated_scan_fwd_kernel<T, TA, sizeof(T) == 4 ? 8 : 16, V, V, false>, grid, block, 0, stream, a);
+    if constexpr (can_row)
+      if (row) return launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, true>, grid, block, 0, stream, a);
     if constexpr (can_share)
-      if (!own)
-        return row ? launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, true>, grid, block, 0, stream, a)
-                   : launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, false>, grid, block, 0, stream, a);
+      if (!own && !row) return launch(gated_scan_fwd_kernel<T, TA, 16, V, 1, false>, grid, block, 0, stream, a);
     return err;
   } else {
     if constexpr (can_own)
       if (own) err = launch(gated_scan_bwd_kernel<T, TA, 8, V, V, false, false>, grid, block, 0, stream, a);
+    if constexpr (can_row)
+      if (row) err = launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, true>, grid, block, 0, stream, a);
     if constexpr (can_share)
-      if (!own)
-        err = row ? launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, true>, grid, block, 0, stream, a)
-                  : launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, false>, grid, block, 0, stream, a);
+      if (!own && !row) err = launch(gated_scan_bwd_kernel<T, TA, 8, V, 1, true, false>, grid, block, 0, stream, a);
     if (err || p.segs == 1) return err;
     const int64_t sums = (int64_t)a.T * a.B * a.G;
     return launch(gated_scan_bwd_finish_kernel<TA>, dim3((unsigned)((sums + 255) / 256)), dim3(256), 0, stream, a, p.segs);

@@ -14,12 +14,6 @@ namespace socmx {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-// include/socmx.h: SOCMX_F32, SOCMX_BF16, SOCMX_F16
-template <int KIND> struct elem_of;
-template <> struct elem_of<0> { typedef float type; };
-template <> struct elem_of<1> { typedef bf16_t type; };
-template <> struct elem_of<2> { typedef f16_t type; };
-
 template <typename T, int N>
 struct mem_vec {
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));

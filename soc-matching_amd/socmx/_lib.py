@@ -45,9 +45,6 @@ class Control(C.Structure):
 
 CTRL_LINEAR, CTRL_CONSTANT, CTRL_TABLE = 1, 2, 3
 
-# element types of the layer operators (include/socmx.h: SOCMX_F32, SOCMX_BF16, SOCMX_F16)
-ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
 
 class Scan(C.Structure):
     _fields_ = [("type", C.c_int32), ("gate_type", C.c_int32), ("T", C.c_int32), ("B", C.c_int32), ("D", C.c_int32),
