@@ -436,3 +436,41 @@ def test_adamw_refuses_tangents():
         for name in ("params", "grads", "exp_avgs", "exp_avg_sqs"):
             with pytest.raises(SocmxError, match="forward-mode"):
                 optim.adamw_step(**{**ok, name: [fwad.make_dual(f(), f())]})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [1e-18, 1e-19])
+def test_adamw_of_tiny_gradients_without_eps_in_codes(bits, size):
+    """eps below 1e-10, states in 32 and in 8 bits: the first update is lr whatever the gradient's size.  v = 0.05 g^2 is 5e-38 at 1e-18 and, at
+    1e-19, 5e-40, 3.6e5 of float32's smallest numbers: off by half of one in g g, its product and the sum, 4.2e-6 of v, half of that of its root."""
+    p, q = torch.zeros(300, device=DEV), torch.full((300,), size, device=DEV)
+    m, v, scales, _ = new_states([300], F32, bits, False, [p])
+    optim.adamw_step([p], [q], m, v, torch.zeros(1, device=DEV), lr=1e-2, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0, scales=scales)
+    close(p, torch.full((300,), -1e-2).double(), 1e-2 * (30 * U + (2.1e-6 if size < 1e-18 else 0)))
+
+
+def test_the_trainer_s_captured_iteration_with_adamw_is_the_eager_one():
+    """Six iterations on the noise of the same device key, replayed and eager: the same losses and the same parameters up to what the two
+    bodies' gradients differ by in their last bits.  (Both are stepped by the same kernel; an entry whose gradient nearly cancels moves by that
+    difference over eps = 1e-4: 1e-5 of an update each, at most lr.)"""
+    from test_host_cpu import build_sde
+    from SOC_matching.method import SOC_Solver
+    from socmx.rollout import PhiloxKey
+    from socmx.train import Trainer, make_optimizer
+    runs = []
+    for graph in (False, True):
+        torch.manual_seed(0)
+        sde, aux = build_sde("tiny_double_well_d10", DEV)
+        solver = SOC_Solver(sde, aux["x0"], None, T=aux["T"], num_steps=aux["K"], lmbd=aux["lmbd"], d=aux["d"], sigma=sde.sigma)
+        solver.philox_key = PhiloxKey(torch.device(DEV), seed=77, offset=5)
+        opt = make_optimizer(solver, nabla_V_lr=1e-3, M_lr=1e-3, weight_decay=0.05, state_bits=32)
+        tr = Trainer(solver, opt, 16, normalization_const=0.8, hip_graph=graph, overlap_M_backward=False)
+        steps = [tr.step() for _ in range(6)]
+        tr.join()
+        torch.cuda.synchronize()
+        runs.append(([float(s["loss"]) for s in steps], {n: p.detach().clone() for n, p in sde.named_parameters()}, [s["mode"] for s in steps]))
+    (le, pe, _), (lg, pg, modes) = runs
+    assert "graph-replay" in modes
+    assert all(abs(a - b) <= 2e-5 * abs(b) + 1e-7 for a, b in zip(lg, le)), (lg, le)
+    for n in pe:
+        close(pg[n], pe[n], 2e-5 * pe[n].abs().double().cpu() + 6 * 1e-5 * 1e-3 + 5e-7)
