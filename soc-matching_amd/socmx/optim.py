@@ -65,6 +65,10 @@ class AdamW(torch.optim.Optimizer):
             raise SocmxError(f"AdamW: parameters on the GPU are needed, got {p.device} (there is no CPU path)")
         if torch.cuda.is_current_stream_capturing():
             raise SocmxError("AdamW: the state of a parameter would be created inside a capture: take one step before it")
+        if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise SocmxError(f"AdamW: float32, bfloat16 or float16 parameters are needed, got {p.dtype}")
+        if torch.empty_like(p).stride() != p.stride() and not p.is_contiguous():
+            raise SocmxError(f"AdamW: a parameter is dense in memory, got strides {p.stride()} for {tuple(p.shape)}")
         st = self.state[p]
         st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
         kinds = (torch.float32, torch.float32) if group["state_bits"] == 32 else (torch.int8, torch.uint8)
@@ -105,19 +109,19 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            kinds = {}
+        found = {}                                 # (what is refused is refused before anything is updated)
+        for k, group in enumerate(self.param_groups):
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise SocmxError("AdamW: a sparse gradient")
                 st = self.state.get(p) or self._new_state(p, group)
-                kinds.setdefault((p.dtype, p.device, "scale" in st, "master" in st), []).append((p, st))
-            for (_, _, small, master), found in kinds.items():
-                adamw_step([p for p, _ in found], [self._laid_like(p.grad, p) for p, _ in found],
-                           [st["exp_avg"] for _, st in found], [st["exp_avg_sq"] for _, st in found], [st["step"] for _, st in found],
-                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           scales=[st["scale"] for _, st in found] if small else None,
-                           masters=[st["master"] for _, st in found] if master else None)
+                found.setdefault((k, p.dtype, p.device, "scale" in st, "master" in st), []).append((p, st))
+        for (k, _, _, small, master), some in found.items():
+            group = self.param_groups[k]
+            adamw_step([p for p, _ in some], [self._laid_like(p.grad, p) for p, _ in some], [st["exp_avg"] for _, st in some],
+                       [st["exp_avg_sq"] for _, st in some], [st["step"] for _, st in some], lr=group["lr"], betas=group["betas"],
+                       eps=group["eps"], weight_decay=group["weight_decay"], scales=[st["scale"] for _, st in some] if small else None,
+                       masters=[st["master"] for _, st in some] if master else None)
         return loss

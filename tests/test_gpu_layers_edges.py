@@ -474,3 +474,25 @@ def test_the_trainer_s_captured_iteration_with_adamw_is_the_eager_one():
     assert all(abs(a - b) <= 2e-5 * abs(b) + 1e-7 for a, b in zip(lg, le)), (lg, le)
     for n in pe:
         close(pg[n], pe[n], 2e-5 * pe[n].abs().double().cpu() + 6 * 1e-5 * 1e-3 + 5e-7)
+
+
+def test_adamw_refuses_before_it_updates_anything():
+    """A parameter that the update has no form for, in the last group: the others stay as they are, and no state is left behind."""
+    good = [torch.nn.Parameter(torch.ones(40, device=DEV)) for _ in range(2)]
+    sparse = torch.nn.Embedding(5, 8, sparse=True, device=DEV)
+    sparse(torch.tensor([1], device=DEV)).sum().backward()
+    for bad in (torch.nn.Parameter(torch.ones(6, 8, device=DEV)[:, ::2]), torch.nn.Parameter(torch.ones(5, dtype=torch.float64, device=DEV)),
+                torch.nn.Parameter(torch.ones(3, 1, device=DEV).expand(3, 4)), sparse.weight, torch.nn.Parameter(torch.ones(5))):
+        if bad.grad is None:
+            bad.grad = torch.ones_like(bad)
+        opt = optim.AdamW([dict(params=good[:1]), dict(params=good[1:], lr=1.0), dict(params=[bad])])
+        for p in good:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(SocmxError):
+            opt.step()
+        assert all(bool((p == 1).all()) for p in good) and bad not in opt.state
+        opt.param_groups[2]["params"] = []
+        opt.step()
+        assert all(float(opt.state[p]["step"]) == 1.0 for p in good)
+        for p in good:
+            p.data.fill_(1.0)
