@@ -10,6 +10,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
@@ -18,6 +19,7 @@
 
 #include <algorithm>
 #include <sstream>
+#include <unordered_set>
 
 #include "../../include/socmx.h"
 
@@ -133,24 +135,34 @@ struct Launch {
   }
 };
 
-bool capturing(const at::Device& dev) {
+bool capturing(void* stream) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  const Launch l(dev);
-  return hipStreamIsCapturing(static_cast<hipStream_t>(l.stream), &s) == hipSuccess && s != hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(static_cast<hipStream_t>(stream), &s) == hipSuccess && s != hipStreamCaptureStatusNone;
 }
+// (the default stream is never captured, and not asked while another one is)
+bool joined(const c10::Stream& s) { return s.id() != 0 && capturing(c10::hip::HIPStreamMasqueradingAsCUDA(s).stream()); }
 
 // A leaf's gradient node keeps the stream of the first autograd graph that used the leaf, for as long as any graph of it lives.  torch
 // makes that stream wait for a backward on another one; inside a capture that draws it into the graph, and closing the capture ends
-// the process.  Such a forward is refused while it is captured, before there is a backward.
+// the process.  Such a forward is refused while it is captured, before there is a backward: for every leaf that leads to its inputs, by
+// whatever operations.
 void refuse_foreign_leaves(const char* what, const at::Device& dev, std::initializer_list<Tensor> inputs) {
-  if (!at::GradMode::is_enabled() || !capturing(dev)) return;
+  if (!at::GradMode::is_enabled() || !capturing(Launch(dev).stream)) return;
   const c10::Stream here = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
-  for (const Tensor& t : inputs) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) continue;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  auto visit = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+    if (node && seen.insert(node.get()).second) todo.push_back(node);
+  };
+  for (const Tensor& t : inputs)
+    if (t.defined() && t.requires_grad()) visit(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+  while (!todo.empty()) {
+    const auto node = todo.back();
+    todo.pop_back();
+    for (const auto& edge : node->next_edges()) visit(edge.function);
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) continue;
     const auto first = node->stream();
-    if (first && *first != here)
+    if (first && *first != here && !joined(*first))
       refuse(what, ": an autograd graph of the same leaf, built on another stream, is alive: drop what keeps it (the outputs of an eager "
                    "iteration) before capturing");
   }

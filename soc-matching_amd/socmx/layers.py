@@ -10,7 +10,8 @@ uses the graph's own memory) and is bit-reproducible: no atomics.  There is no C
 
 Gradients inside a captured graph: no autograd graph of the same leaves that was built on another stream may be alive (an output kept
 from an eager iteration).  torch ties a leaf's gradient to the stream of its first graph and would wait for the capture there, which
-ends the process when the capture is closed; a call that is captured in that state raises SocmxError instead.
+ends the process when the capture is closed; a call that is captured while a leaf that leads to it is in that state raises SocmxError
+instead.  (Leaves that are used behind the call are not seen by it.)
 
 Derivatives are reverse-mode and first order: an input with a forward-mode tangent raises SocmxError, a second derivative raises RuntimeError.
 A call under torch.jit.trace or make_fx raises SocmxError.

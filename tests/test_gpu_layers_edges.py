@@ -3,6 +3,7 @@ infinite, gradients of gradients, rows far from zero, memory that is shared, gra
 
 Oracles are plain formulas in 64 bits; tolerances count roundings in units of U = 2^-24, as in test_gpu_layers.py.
 """
+import gc
 import math
 
 import pytest
@@ -496,3 +497,58 @@ def test_adamw_refuses_before_it_updates_anything():
         assert all(float(opt.state[p]["step"]) == 1.0 for p in good)
         for p in good:
             p.data.fill_(1.0)
+
+
+def test_a_capture_is_refused_for_every_leaf_that_leads_to_the_call():
+    """Not only for leaves that are inputs themselves.  A leaf first used on a stream that the capture has joined is none of these."""
+    d = 12
+    net = torch.nn.Linear(d, d, device=DEV)
+    x = torch.randn(5, 3, d, device=DEV)
+    decay = torch.full((1, 1, 2), -0.5, device=DEV, requires_grad=True)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def forward(which):
+        y = torch.tanh(net(x)) * 2
+        if which == "norm":
+            return layers.layer_norm(y)
+        return layers.gated_scan(x if which == "decay" else y, (decay * 2).expand(5, 3, 2))[0]
+    for which in ("norm", "scan", "decay"):
+        alive = forward(which)                                 # on the current stream
+        side.wait_stream(torch.cuda.current_stream())
+        with pytest.raises(SocmxError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                forward(which)                                 # (refused before there is a backward)
+        del alive
+        gc.collect()                                           # (frames of the refused call)
+    params = list(net.parameters()) + [decay]
+
+    def step(out):
+        for p, q in zip(params, torch.autograd.grad(out, params, torch.ones_like(out))):
+            p.grad = q
+    want = forward("scan")
+    step(want)
+    eager, want = [p.grad.clone() for p in params], want.detach().clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):                              # (libraries set themselves up outside the capture)
+        for _ in range(2):
+            step(forward("scan"))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            y = torch.tanh(net(x)) * 2                         # a branch of the capture
+        side.wait_stream(other)
+        out = layers.gated_scan(y, (decay * 2).expand(5, 3, 2))[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del out, y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(forward("scan"))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        forward("norm").sum().item()
+        assert all(torch.allclose(p.grad, q, rtol=1e-5, atol=1e-6) for p, q in zip(params, eager))
