@@ -578,8 +578,8 @@ int socmx_layer_norm_bwd(int32_t type, int32_t wtype, const void* x, int64_t row
  *   (B, D) f32 dense, each may be NULL.  lengths (B,) int32 device or NULL: row b has min(max(lengths[b], 0), T) steps; the steps behind
  *   them are not read, their h, dx and dlog_decay are 0 and the final state is the one before them.  reverse: from a row's last step
  *   to its first.  A decay of 0 (log_decay = -inf, or so low that exp is below 2^-126) forgets all before it, infinities and
- *   NaN included.  A state that is infinite under other decays stays no finite number, but may become a NaN; the steps behind a row's
- *   length leave it infinite.
+ *   NaN included.  A state that is infinite under other decays stays no finite number, but may become a NaN (log_decay from
+ *   -1/4 to 0); the steps behind a row's length leave it infinite.
  * states: socmx_gated_scan_sizes state_floats of f32, kept from the forward for the backward (NULL when none follows).  Workspaces: floats
  *   as socmx_gated_scan_sizes says (NULL where 0; at a multiple of 8 bytes), contents undefined before and after, one for each call in
  *   flight.

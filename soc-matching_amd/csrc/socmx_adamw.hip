@@ -17,9 +17,10 @@
 // than the same formula elsewhere.  A positive v never becomes 0: eps alone would divide m.
 // The weight's update uses m and v as they are before they are rounded.  A block with a value that is not finite gets a NaN scale.
 //
-// MEASURED, 96 M elements: f32 weights, 32 bits 547 us (4.9 TB/s, the rate of a copy of this size); bf16 weights with f32 masters, 8 bits
-// 363 us (4.2 TB/s, a copy of as many bytes 314; arithmetic, 116 instructions an element, issues for 280 of them); their decoded values 166
-// us (5.8 TB/s, most of it stores).  Stores past the caches cost 4 %.  18 tensors, 171 k elements: 6 us.
+// MEASURED, 96 M elements: 32 bits, f32 weights 519 us in 24 tensors (5.2 TB/s) and 547 in 100 at odd offsets (4.9, the rate of a copy of this size),
+// bf16 404 (5.2), with f32 masters 513 (5.2).  8 bits: f32 326 to 356, bf16 298 to 327, with masters 337 to 391 (4.6 to 3.9 TB/s; a copy of as many
+// bytes 314): arithmetic, 118 instructions an element, issues for 285 us of it, bf16 without masters moves its bytes in 190.  Their decoded
+// values 161 us (6.0 TB/s, most of it stores).  Stores past the caches cost 4 %.  18 tensors, 171 k elements: 6.4 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -14,10 +14,11 @@
 // their own and a second launch adds the slots in a fixed order: no atomics, the same bits on every run.  Rows of more than
 // 16384 elements are read again from the caches instead of being kept (the *_long kernels).
 //
-// MEASURED.  bf16 (8192, 4096): forward 26.5 us (5.1 TB/s), backward 40 (5.0) and 4 for the slots, a copy of this size runs at 5.3 to 6.8;
-// f32 (25728, 256): 11 (4.8), 16 (4.9) and 3.  f16 (4111, 1601), rows at odd addresses: 12, 16 and 5, a third of that rate: one row a workgroup,
-// all of them at once, so what is left is the way of one row through three sums.  y leaves past the caches (28.5 -> 26.5 us); dx did not gain.
-// The first shape's forward with 8 elements a lane (twice the waves a row) 30 us, with 32 28, alone 24.6; (4111, 1601) 11.0, 13.6 and 10.8.
+// MEASURED.  bf16 (8192, 4096): forward 27.5 us (4.9 TB/s), backward 41.5 (4.9; 40 without the sum of n) and 4 for the slots, a copy of this size runs
+// at 5.3 to 6.8; f32 (25728, 256): 11 (4.8), 16.5 (4.8) and 3.6; f32 (4096, 12288): 91 (4.4), 105 (5.8) and 6.  f16 (4111, 1601), y, dy and dx at odd
+// addresses: 12, 17 and 5.5, a third of that rate: one row a workgroup at a time, so what is left is the way of one row through its sums, and
+// in the backward the slots.  y leaves past the caches (28.5 -> 26.5 us); dx did not gain.  The first shape's forward with 8 elements a lane
+// (twice the waves a row) 30 us, with 32 28, alone 24.6; (4111, 1601) 11.0, 13.6 and 10.8.  bf16 (512, 50000): 34, 42, 21.5 and 10.6.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -375,8 +376,8 @@ static inline int norm_lanes(int cols, int vec) {
   return lanes;
 }
 
-// the backward's workgroups, each with a slot of weight gradients: enough rows for each that the slots are a small part of the
-// traffic, two workgroups' worth of waves for every CU at most
+// the backward's workgroups, each with a slot of weight gradients: eight waves for every CU at most (a workgroup for every CU at least).  What the
+// slots add to the rows' traffic, written and read: 3 % for (25728, 256) f32, 17 % for (8192, 4096) bf16, 66 % for (4111, 1601) f16, 4 rows a slot
 static inline int64_t norm_slots(int64_t rows, int cols, int vec) {
   if (cols > kNormKept) return std::min<int64_t>(rows, 64);
   const int lanes = norm_lanes(cols, vec), groups = lanes <= 64 ? 256 / lanes : 1;

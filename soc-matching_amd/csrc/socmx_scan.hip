@@ -27,9 +27,10 @@
 // products are summed across the lanes in a fixed order, gates wider than a wave leave one partial sum a wave for another launch.  No
 // floating-point atomics.
 //
-// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 116 us (4.4 TB/s of x, alpha, h and states) + 163 us (5.2): memory, a copy of
-// this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 70 us (4.1 TB/s) + 123 us (3.5); rows of 0 to 4096 steps, 55 % of them in
-// all, 62 + 96 (3.7, 3.2), of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 13 + 23.  Results leave past the caches (5 % less than through them).
+// MEASURED (forward + backward): f32 (65536, 1, 640), a decay each: 112 to 121 us (4.2 to 4.6 TB/s of x, alpha, h and states) + 158 to 168 us (5.1 to 5.4):
+// memory, a copy of this size runs at 4.9.  bf16 (4096, 8, 2048), 32 decays a step: 63 us (4.6 TB/s) + 103 us (4.1); rows of 0 to 4096 steps, 55 % of
+// them in all, 60 + 95 (3.8, 3.2), of which arithmetic is 20 + 32.  f32 (201, 128, 256), 8 decays: 14 + 21.  Results leave past the caches (5 % less
+// than through them).
 // Reading x and alpha twice -- once for the runs, once for the steps, in launches of their own -- took 447, 238 and 57 us together.  U = 16 was the
 // best among 4, 8, 16; chunks wait for each other 3 to 7 % of the time.  Workgroups that stay and draw their next ticket early hold up
 // whoever waits for it: 283 -> 315 us for the first shape.

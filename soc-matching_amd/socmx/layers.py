@@ -59,7 +59,8 @@ def gated_scan(x, log_decay, initial=None, lengths=None, reverse=False):
     lengths (B,) int32: row b's steps are the first lengths[b] (0 to T; values outside are clipped); the steps behind them are not
     read, their h and gradients are 0 and the final state is the one before them.  reverse: from each row's last step to its
     first.  The state and all sums are float32 whatever x's type; a state that grows (log_decay above 0) beyond float32 is infinite or NaN, also
-    where the growth of up to 256 steps together is beyond it and the state is not zero.  Differentiable in x, log_decay and initial."""
+    where the growth of up to 256 steps together is beyond it and the state is not zero; an infinite one may become NaN under a log_decay
+    from -1/4 to 0, the steps behind a row's length leave it as it is.  Differentiable in x, log_decay and initial."""
     return _binding().gated_scan(x, log_decay, initial, lengths, reverse)
 
 

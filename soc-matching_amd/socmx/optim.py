@@ -44,7 +44,8 @@ def adamw_state_values(exp_avgs, exp_avg_sqs, scales):
 class AdamW(torch.optim.Optimizer):
     """AdamW whose step is one call of `adamw_step` for each type of weights in a group (48 tensors a launch).
 
-    state_bits: 32 (float32 states) or 8 (one byte a state, two float32 for 256 elements).  master_weights: keep float32 weights for 16-bit
+    state_bits: 32 (float32 states) or 8 (one byte a state, two float32 for 256 elements: a gradient that is not finite makes the states of all 256
+    NaN from then on, and their weights with the next step).  master_weights: keep float32 weights for 16-bit
     parameters (a 16-bit weight does not see updates below 2^-9 of it).  The state is that of torch.optim.AdamW -- "step", "exp_avg",
     "exp_avg_sq" -- and, where there are any, "scale" and "master".  Parameters without a gradient are left alone.  The state of a
     parameter, its step count included, lives on the GPU and stays where it is, so step() can be captured in a graph once the state exists (one
