@@ -135,19 +135,25 @@ struct Launch {
   }
 };
 
-bool capturing(void* stream) {
+// the number of the capture that a stream is part of, or 0
+unsigned long long capture_of(void* stream) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(static_cast<hipStream_t>(stream), &s) == hipSuccess && s != hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  return hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &s, &id) == hipSuccess && s == hipStreamCaptureStatusActive ? id : 0;
 }
 // (the default stream is never captured, and not asked while another one is)
-bool joined(const c10::Stream& s) { return s.id() != 0 && capturing(c10::hip::HIPStreamMasqueradingAsCUDA(s).stream()); }
+bool joined(const c10::Stream& s, unsigned long long capture) {
+  return s.id() != 0 && capture_of(c10::hip::HIPStreamMasqueradingAsCUDA(s).stream()) == capture;
+}
 
 // A leaf's gradient node keeps the stream of the first autograd graph that used the leaf, for as long as any graph of it lives.  torch
 // makes that stream wait for a backward on another one; inside a capture that draws it into the graph, and closing the capture ends
 // the process.  Such a forward is refused while it is captured, before there is a backward: for every leaf that leads to its inputs, by
 // whatever operations.
 void refuse_foreign_leaves(const char* what, const at::Device& dev, std::initializer_list<Tensor> inputs) {
-  if (!at::GradMode::is_enabled() || !capturing(Launch(dev).stream)) return;
+  if (!at::GradMode::is_enabled()) return;
+  const unsigned long long capture = capture_of(Launch(dev).stream);
+  if (capture == 0) return;
   const c10::Stream here = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
   std::vector<std::shared_ptr<torch::autograd::Node>> todo;
   std::unordered_set<torch::autograd::Node*> seen;
@@ -162,7 +168,7 @@ void refuse_foreign_leaves(const char* what, const at::Device& dev, std::initial
     for (const auto& edge : node->next_edges()) visit(edge.function);
     if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) continue;
     const auto first = node->stream();
-    if (first && *first != here && !joined(*first))
+    if (first && *first != here && !joined(*first, capture))
       refuse(what, ": an autograd graph of the same leaf, built on another stream, is alive: drop what keeps it (the outputs of an eager "
                    "iteration) before capturing");
   }
